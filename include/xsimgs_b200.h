@@ -525,6 +525,70 @@ int xsg_nvls_broadcast_f32(const float* src, uint64_t mc_dst, int64_t n, xsg_str
 /* At most n CTAs per exchange kernel (0: four per SM, the default). */
 void xsg_exchange_set_max_ctas(int n);
 
+/* ---- the end of a training step (no reference counterpart: the reference
+ * leaves the optimiser to its caller) ----
+ * Many tensors in one call.  Arrays named *_host are read before the call
+ * returns; the tensors they point to are on the device, dense (any order of
+ * dimensions, no gaps), aligned to their element, and may be of any length,
+ * zero included.  The sum of all lengths is below 2^40.  Sums are held in 64
+ * bits and taken in an order that depends on the lengths alone. */
+enum xsg_dtype {
+    XSG_F32 = 0,
+    XSG_BF16 = 1,
+    XSG_F16 = 2,
+};
+enum xsg_norm_type {
+    XSG_NORM_INF = 0,
+    XSG_NORM_1 = 1,
+    XSG_NORM_2 = 2,
+};
+typedef struct xsg_span {
+    void* data;
+    int64_t n;     /* elements */
+    int32_t dtype; /* xsg_dtype */
+} xsg_span;
+/* Scratch of the three calls below. */
+size_t xsg_grad_norm_workspace_size(int64_t n_spans);
+/* norm [1] = the norm of all elements of all tensors; norms [n_spans] (may be
+ * NULL) = each tensor's.  NaN and infinite elements give a NaN or infinite
+ * norm. */
+int xsg_grad_norm(const xsg_span* spans_host, int64_t n_spans, int norm_type, float* norm, float* norms,
+                  void* workspace, size_t workspace_bytes, xsg_stream_t stream);
+/* norm [1] as above; every element is multiplied by
+ * min(1, max_norm / (norm + 1e-6)), in 32 bits, rounded once.  An infinite
+ * norm scales by 0, a NaN makes every element NaN.  No two tensors may share
+ * memory. */
+int xsg_clip_grads(const xsg_span* spans_host, int64_t n_spans, int norm_type, float max_norm, float* norm,
+                   void* workspace, size_t workspace_bytes, xsg_stream_t stream);
+/* One tensor of an AdamW update.  master (may be NULL): the 32-bit parameter
+ * that `param` is a rounding of.  row_mask (may be NULL): n / row_size bytes,
+ * rows of zero stay as they are (parameter and moments). */
+typedef struct xsg_adamw_span {
+    void* param;
+    const void* grad;
+    float* exp_avg;
+    float* exp_avg_sq;
+    float* master;
+    const uint8_t* row_mask;
+    int64_t n;
+    int64_t row_size;
+    int32_t param_dtype; /* xsg_dtype */
+    int32_t grad_dtype;
+    double lr, beta1, beta2, eps, weight_decay;
+} xsg_adamw_span;
+/* step [2]: the number of updates taken so far, which the call advances by
+ * one, and a word that is zero between calls.  With t = step + 1:
+ *   g' = c g, m <- b1 m + (1 - b1) g', v <- b2 v + (1 - b2) g'^2,
+ *   w <- w - lr wd w - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps).
+ * max_norm >= 0: c is the clipping coefficient of all gradients' 2-norm (the
+ * gradients themselves stay as they are); below 0: c = 1.  skip_nonfinite: a
+ * norm that is NaN or infinite leaves everything as it was, `step` too.
+ * norm [1] (may be NULL): the 2-norm.  The workspace is needed for any of the
+ * three.  No two written tensors may share memory. */
+int xsg_adamw_update(const xsg_adamw_span* spans_host, int64_t n_spans, int64_t* step, float max_norm,
+                     int skip_nonfinite, float* norm, void* workspace, size_t workspace_bytes,
+                     xsg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,117 @@
+"""CPU checks of the gradient norm, clipping and AdamW entries: refusals that
+happen before any CUDA call, through the extension and the C ABI."""
+import ctypes as C
+import inspect
+
+import pytest
+import torch
+
+
+class Span(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("n", C.c_int64), ("dtype", C.c_int32)]
+
+
+class AdamSpan(C.Structure):
+    _fields_ = [(k, C.c_void_p) for k in ("param", "grad", "exp_avg", "exp_avg_sq", "master", "row_mask")] + \
+               [("n", C.c_int64), ("row_size", C.c_int64), ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32)] + \
+               [(k, C.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from xsimgs_b200 import capi
+    lib = capi.lib()
+    lib.xsg_grad_norm_workspace_size.restype = C.c_size_t
+    lib.xsg_grad_norm_workspace_size.argtypes = [C.c_int64]
+    return lib
+
+
+def test_workspace_size(lib):
+    size = lib.xsg_grad_norm_workspace_size
+    assert size(0) == 0 and size(-3) == 0
+    assert 0 < size(1) <= size(1000) <= size(5000) < 1 << 20
+
+
+def refuse(lib, rc, code, text):
+    assert rc == code and text in lib.xsg_last_error(), (rc, lib.xsg_last_error())
+
+
+def test_c_abi_refusals(lib):
+    fake = 1 << 20  # never read: every call below is refused before a launch
+    one = (Span * 1)(Span(fake, 8, 0))
+
+    def norm(spans=one, n=1, p=2, out=fake, ws=fake, size=1 << 20):
+        return lib.xsg_grad_norm(spans, C.c_int64(n), p, C.c_void_p(out), None, C.c_void_p(ws), C.c_size_t(size), None)
+
+    refuse(lib, norm(n=0), 1, b"at least one tensor")
+    refuse(lib, norm(spans=None), 1, b"at least one tensor")
+    refuse(lib, norm(out=None), 1, b"null output")
+    refuse(lib, norm(p=3), 1, b"norm type")
+    refuse(lib, norm(ws=None), 4, b"workspace")
+    refuse(lib, norm(size=8), 4, b"workspace")
+    refuse(lib, norm(spans=(Span * 1)(Span(fake, -1, 0))), 1, b"element count")
+    refuse(lib, norm(spans=(Span * 1)(Span(fake, 1 << 40, 0))), 1, b"element count")
+    refuse(lib, norm(spans=(Span * 1)(Span(None, 4, 0))), 1, b"null pointer")
+    refuse(lib, norm(spans=(Span * 1)(Span(fake + 2, 4, 0))), 1, b"misaligned")
+    refuse(lib, norm(spans=(Span * 1)(Span(fake, 4, 7))), 1, b"element type")
+
+    def clip(limit):
+        return lib.xsg_clip_grads(one, C.c_int64(1), 2, C.c_float(limit), C.c_void_p(fake), C.c_void_p(fake),
+                                  C.c_size_t(1 << 20), None)
+
+    for bad in (-1.0, float("inf"), float("nan")):
+        refuse(lib, clip(bad), 1, b"max_norm")
+
+    def adamw(step=fake, ws=fake, max_norm=-1.0, **kw):
+        f = dict(param=fake, grad=fake, exp_avg=fake, exp_avg_sq=fake, n=8, lr=0.1, beta1=0.9, beta2=0.99, eps=1e-8)
+        f.update(kw)
+        s = (AdamSpan * 1)(AdamSpan(**f))
+        return lib.xsg_adamw_update(s, C.c_int64(1), C.c_void_p(step), C.c_float(max_norm), 0, None, C.c_void_p(ws),
+                                    C.c_size_t(1 << 20 if ws else 0), None)
+
+    refuse(lib, adamw(step=None), 1, b"step counter")
+    refuse(lib, adamw(param=None), 1, b"null pointer")
+    refuse(lib, adamw(grad=fake + 1), 1, b"misaligned")
+    refuse(lib, adamw(exp_avg=fake + 2), 1, b"misaligned")
+    refuse(lib, adamw(param_dtype=5), 1, b"element type")
+    refuse(lib, adamw(n=-2), 1, b"element count")
+    refuse(lib, adamw(row_mask=fake), 1, b"row size")
+    refuse(lib, adamw(beta1=1.0), 1, b"betas")
+    refuse(lib, adamw(beta2=-0.1), 1, b"betas")
+    refuse(lib, adamw(eps=-1.0), 1, b"eps")
+    refuse(lib, adamw(lr=float("nan")), 1, b"learning rate")
+    refuse(lib, adamw(max_norm=float("inf")), 1, b"max_norm")
+    refuse(lib, adamw(max_norm=1.0, ws=None), 4, b"workspace")
+
+
+def test_extension_refusals_without_gpu():
+    import xsimgs_b200 as X
+    t = torch.zeros(4)
+    step = X.adamw_step_counter("cpu", 3)
+    assert step.tolist() == [3, 0]
+    for call, match in [
+        (lambda: X.gradient_norm([]), "at least one"),
+        (lambda: X.gradient_norm([t]), "CUDA"),
+        (lambda: X.clip_gradients_([], 1.0), "at least one"),
+        (lambda: X.clip_gradients_([t], 1.0), "CUDA"),
+        (lambda: X.clip_gradients_([t], -1.0), "max_norm"),
+        (lambda: X.gradient_norm([t], norm_type=0.5), "norm_type"),
+        (lambda: X.adamw_update_([], [], [], [], step, lr=0.1), "at least one"),
+        (lambda: X.adamw_update_([t], [t], [t], [t], step, lr=0.1), "CUDA"),
+        (lambda: X.adamw_update_([t], [], [t], [t], step, lr=0.1), "same length"),
+        (lambda: X.adamw_update_([t], [t], [t], [t], step, lr=[0.1, 0.2, 0.3]), "one value"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            call()
+
+
+def test_optimizer_arguments():
+    import xsimgs_b200 as X
+    p = torch.zeros(3, requires_grad=True)
+    for bad in (dict(lr=-1.0), dict(eps=-1e-8), dict(weight_decay=-0.1), dict(betas=(0.9, 1.0))):
+        with pytest.raises(ValueError):
+            X.AdamW([p], **bad)
+    opt = X.AdamW([dict(params=[p], lr=0.5)], lr=0.1, betas=(0.8, 0.9))
+    assert opt.param_groups[0]["lr"] == 0.5 and opt.param_groups[0]["betas"] == (0.8, 0.9)
+    assert opt.step() is None  # no gradients: nothing to do
+    assert "row_masks" in inspect.signature(opt.step).parameters

@@ -12,6 +12,9 @@ from .rendering import (  # noqa: F401
     ut_gs_render, ut_gs_tiling, ut_gs_rasterize, ut_gs_dynamic_rasterize,
     spherical_harmonics_fused, rgb_to_sh0, sh0_to_rgb, sh_degree_to_bands,
 )
+from .optim import (  # noqa: F401
+    gradient_norm, clip_gradients_, adamw_update_, adamw_step_counter, AdamW,
+)
 from . import cameras  # noqa: F401
 
 __version__ = "0.1.0"

@@ -8,6 +8,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
+#include <limits>
 #include <optional>
 #include <string>
 #include <vector>
@@ -914,6 +917,225 @@ std::tuple<Tensor, Tensor, Tensor> interpolate_smpl_bwd(const Tensor& poses, con
     return {d_poses, d_root, d_q};
 }
 
+// ------------------------------------------- the end of a training step --
+int dtype_code(const Tensor& t, const char* name) {
+    switch (t.scalar_type()) {
+        case at::kFloat: return XSG_F32;
+        case at::kBFloat16: return XSG_BF16;
+        case at::kHalf: return XSG_F16;
+        default: TORCH_CHECK(false, name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+    }
+}
+
+void check_listed(const Tensor& t, const char* name, const Tensor& ref) {
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided, name, " must be dense tensors");
+    require_cuda(t, name);
+    TORCH_CHECK(t.device() == ref.device(), name, " must all be on one device, got ", t.device(), " and ",
+                ref.device());
+}
+
+// A tensor that is written has to own its elements: every one at an address
+// of its own, without gaps.
+void check_written(const Tensor& t, const char* name, const Tensor& ref) {
+    check_listed(t, name, ref);
+    TORCH_CHECK(t.is_non_overlapping_and_dense(), name, " must be dense (no gaps, no expanded dimensions): got sizes ",
+                t.sizes(), " with strides ", t.strides());
+}
+
+// Whether two tensors of the same sizes hold their elements in the same order
+// (the strides of dimensions of one element say nothing).
+bool same_order(const Tensor& a, const Tensor& b) {
+    if (a.numel() == 0) return true;
+    for (int64_t d = 0; d < a.dim(); ++d)
+        if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+    return true;
+}
+
+struct Extent {
+    uintptr_t begin, end;
+    bool written;
+};
+
+void add_extent(std::vector<Extent>& e, const Tensor& t, bool written) {
+    if (t.numel() == 0) return;
+    const auto p = reinterpret_cast<uintptr_t>(t.data_ptr());
+    e.push_back({p, p + size_t(t.numel()) * t.element_size(), written});
+}
+
+void check_apart(std::vector<Extent>& e, const char* what) {
+    std::sort(e.begin(), e.end(), [](const Extent& a, const Extent& b) { return a.begin < b.begin; });
+    uintptr_t any = 0, written = 0;
+    for (const Extent& x : e) {
+        TORCH_CHECK(x.begin >= written && !(x.written && x.begin < any), what,
+                    ": a written tensor shares memory with another tensor of the call");
+        any = std::max(any, x.end);
+        if (x.written) written = std::max(written, x.end);
+    }
+}
+
+int norm_code(double p) {
+    if (p == 2.0) return XSG_NORM_2;
+    if (p == 1.0) return XSG_NORM_1;
+    TORCH_CHECK(p == std::numeric_limits<double>::infinity(), "norm_type must be 1, 2 or inf, got ", p);
+    return XSG_NORM_INF;
+}
+
+py::object gradient_norm(const std::vector<Tensor>& grads, double norm_type, bool per_tensor) {
+    TORCH_CHECK(!grads.empty(), "gradient_norm: at least one tensor is needed");
+    const int p = norm_code(norm_type);
+    std::vector<Tensor> copies;  // of tensors with gaps or expanded dimensions
+    std::vector<xsg_span> spans(grads.size());
+    require_cuda(grads[0], "grads");
+    c10::cuda::CUDAGuard g(grads[0].device());
+    for (size_t i = 0; i < grads.size(); ++i) {
+        check_listed(grads[i], "grads", grads[0]);
+        const int dtype = dtype_code(grads[i], "grads");
+        const bool dense = grads[i].is_non_overlapping_and_dense();
+        if (!dense) copies.push_back(grads[i].contiguous());
+        const Tensor& t = dense ? grads[i] : copies.back();
+        spans[i] = {t.data_ptr(), t.numel(), dtype};
+    }
+    const auto f32 = grads[0].options().dtype(at::kFloat).requires_grad(false);
+    Tensor norm = at::empty({}, f32);
+    Tensor norms = per_tensor ? at::empty({int64_t(grads.size())}, f32) : Tensor();
+    Tensor ws = workspace(xsg_grad_norm_workspace_size(int64_t(spans.size())), norm);
+    check(xsg_grad_norm(spans.data(), int64_t(spans.size()), p, fptr_mut(norm), per_tensor ? fptr_mut(norms) : nullptr,
+                        ws.data_ptr(), size_t(ws.nbytes()), stream()));
+    if (per_tensor) return py::make_tuple(norm, norms);
+    return py::cast(norm);
+}
+
+Tensor clip_gradients(const std::vector<Tensor>& grads, double max_norm, double norm_type) {
+    TORCH_CHECK(!grads.empty(), "clip_gradients_: at least one tensor is needed");
+    const int p = norm_code(norm_type);
+    TORCH_CHECK(std::isfinite(max_norm) && max_norm >= 0.0 && max_norm <= std::numeric_limits<float>::max(),
+                "clip_gradients_: max_norm must be finite and not negative, got ", max_norm);
+    std::vector<xsg_span> spans(grads.size());
+    std::vector<Extent> extents;
+    require_cuda(grads[0], "grads");
+    for (size_t i = 0; i < grads.size(); ++i) {
+        check_written(grads[i], "grads", grads[0]);
+        spans[i] = {grads[i].data_ptr(), grads[i].numel(), dtype_code(grads[i], "grads")};
+        add_extent(extents, grads[i], true);
+    }
+    check_apart(extents, "clip_gradients_");
+    c10::cuda::CUDAGuard g(grads[0].device());
+    Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+    Tensor ws = workspace(xsg_grad_norm_workspace_size(int64_t(spans.size())), norm);
+    for (const Tensor& t : grads) torch::autograd::impl::bump_version(t);
+    check(xsg_clip_grads(spans.data(), int64_t(spans.size()), p, float(max_norm), fptr_mut(norm), ws.data_ptr(),
+                         size_t(ws.nbytes()), stream()));
+    return norm;
+}
+
+// One value for all tensors, or one for each.
+double nth(const std::vector<double>& v, size_t i) { return v.size() == 1 ? v[0] : v[i]; }
+
+std::optional<Tensor> adamw_update(const std::vector<Tensor>& params, const std::vector<Tensor>& grads,
+                                   const std::vector<Tensor>& exp_avgs, const std::vector<Tensor>& exp_avg_sqs,
+                                   const Tensor& step, const std::vector<double>& lr, const std::vector<double>& beta1,
+                                   const std::vector<double>& beta2, const std::vector<double>& eps,
+                                   const std::vector<double>& weight_decay, std::optional<double> max_norm,
+                                   bool skip_nonfinite, const std::vector<OptT>& masters,
+                                   const std::vector<OptT>& row_masks) {
+    const size_t n = params.size();
+    TORCH_CHECK(n > 0, "adamw_update_: at least one tensor is needed");
+    TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n,
+                "adamw_update_: params, grads, exp_avgs and exp_avg_sqs must have the same length");
+    TORCH_CHECK((masters.empty() || masters.size() == n), "adamw_update_: masters must have one entry for each param");
+    TORCH_CHECK(row_masks.size() <= 1 || row_masks.size() == n,
+                "adamw_update_: row_mask must be one mask or one entry for each param");
+    for (const auto* v : {&lr, &beta1, &beta2, &eps, &weight_decay})
+        TORCH_CHECK(v->size() == 1 || v->size() == n,
+                    "adamw_update_: lr, betas, eps and weight_decay must be one value or one for each param");
+    TORCH_CHECK(!max_norm || (std::isfinite(*max_norm) && *max_norm >= 0.0 &&
+                              *max_norm <= std::numeric_limits<float>::max()),
+                "adamw_update_: max_norm must be finite and not negative");
+    require_cuda(params[0], "params");
+    check_listed(step, "step", params[0]);
+    TORCH_CHECK(step.scalar_type() == at::kLong && step.numel() == 2 && step.is_contiguous(),
+                "adamw_update_: step must be a contiguous int64 tensor of two words (adamw_step_counter)");
+    c10::cuda::CUDAGuard g(params[0].device());
+    std::vector<xsg_adamw_span> spans(n);
+    std::vector<Tensor> copies;  // of gradients whose order of dimensions is not their parameter's
+    std::vector<Extent> extents;
+    extents.reserve(5 * n + 1);
+    add_extent(extents, step, true);
+    for (size_t i = 0; i < n; ++i) {
+        const Tensor& p = params[i];
+        xsg_adamw_span& s = spans[i];
+        check_written(p, "params", params[0]);
+        const bool has_master = !masters.empty() && has(masters[i]);
+        const Tensor* state[3] = {&exp_avgs[i], &exp_avg_sqs[i], has_master ? &*masters[i] : nullptr};
+        const char* names[3] = {"exp_avgs", "exp_avg_sqs", "masters"};
+        for (int k = 0; k < 3; ++k) {
+            if (!state[k]) continue;
+            check_written(*state[k], names[k], params[0]);
+            require_f32(*state[k], names[k]);
+            TORCH_CHECK(state[k]->sizes() == p.sizes() && same_order(*state[k], p), names[k],
+                        " must have their parameter's sizes and strides");
+            add_extent(extents, *state[k], true);
+        }
+        check_listed(grads[i], "grads", params[0]);
+        TORCH_CHECK(grads[i].sizes() == p.sizes(), "grads must have their parameter's sizes, got ", grads[i].sizes(),
+                    " and ", p.sizes());
+        s.grad_dtype = dtype_code(grads[i], "grads");
+        s.param_dtype = dtype_code(p, "params");
+        const bool same = same_order(grads[i], p);
+        if (!same) copies.push_back(at::empty_strided(p.sizes(), p.strides(), grads[i].options()).copy_(grads[i]));
+        const Tensor& grad = same ? grads[i] : copies.back();
+        add_extent(extents, p, true);
+        add_extent(extents, grad, false);
+        s.param = p.data_ptr();
+        s.grad = grad.data_ptr();
+        s.exp_avg = fptr_mut(exp_avgs[i]);
+        s.exp_avg_sq = fptr_mut(exp_avg_sqs[i]);
+        s.master = has_master ? fptr_mut(*masters[i]) : nullptr;
+        s.n = p.numel();
+        s.row_size = 0;
+        s.row_mask = nullptr;
+        if (!row_masks.empty()) {
+            const OptT& mask = row_masks.size() == 1 ? row_masks[0] : row_masks[i];
+            if (has(mask)) {
+                check_listed(*mask, "row_mask", params[0]);
+                TORCH_CHECK(mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte,
+                            "row_mask must be bool or uint8");
+                TORCH_CHECK(mask->dim() == 1 && mask->is_contiguous(), "row_mask must be one contiguous dimension");
+                TORCH_CHECK(p.dim() >= 1 && p.size(0) == mask->size(0), "row_mask must have one entry for each of the ",
+                            p.dim() >= 1 ? p.size(0) : 0, " rows of its parameter, got ", mask->size(0));
+                TORCH_CHECK(p.is_contiguous(), "params under a row_mask must be contiguous");
+                if (s.n > 0) {
+                    s.row_mask = static_cast<const uint8_t*>(mask->data_ptr());
+                    s.row_size = s.n / p.size(0);
+                    TORCH_CHECK(s.row_size < (int64_t(1) << 30), "adamw_update_: rows under a mask are too long");
+                }
+            }
+        }
+        s.lr = nth(lr, i);
+        s.beta1 = nth(beta1, i);
+        s.beta2 = nth(beta2, i);
+        s.eps = nth(eps, i);
+        s.weight_decay = nth(weight_decay, i);
+    }
+    check_apart(extents, "adamw_update_");
+    const bool normed = max_norm.has_value() || skip_nonfinite;
+    Tensor norm, ws;
+    if (normed) {
+        norm = at::empty({}, params[0].options().dtype(at::kFloat).requires_grad(false));
+        ws = workspace(xsg_grad_norm_workspace_size(int64_t(n)), norm);
+    }
+    for (size_t i = 0; i < n; ++i) {
+        torch::autograd::impl::bump_version(params[i]);
+        torch::autograd::impl::bump_version(exp_avgs[i]);
+        torch::autograd::impl::bump_version(exp_avg_sqs[i]);
+        if (spans[i].master) torch::autograd::impl::bump_version(*masters[i]);
+    }
+    check(xsg_adamw_update(spans.data(), int64_t(n), step.data_ptr<int64_t>(), max_norm ? float(*max_norm) : -1.f,
+                           skip_nonfinite, normed ? fptr_mut(norm) : nullptr, normed ? ws.data_ptr() : nullptr,
+                           normed ? size_t(ws.nbytes()) : 0, stream()));
+    return normed ? std::optional<Tensor>(norm) : std::nullopt;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -1104,4 +1326,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("root_q"), py::arg("instance_ids"), py::arg("query_time"));
     m.def("interpolate_smpl_poses_bwd", &interpolate_smpl_bwd, py::arg("smpl_poses"), py::arg("smpl_poses_time"),
           py::arg("root_q"), py::arg("instance_ids"), py::arg("query_time"), py::arg("grad_out_quats"));
+    m.def("gradient_norm", &gradient_norm, py::arg("grads"), py::arg("norm_type") = 2.0,
+          py::arg("per_tensor") = false);
+    m.def("clip_gradients_", &clip_gradients, py::arg("grads"), py::arg("max_norm"), py::arg("norm_type") = 2.0);
+    m.def("adamw_update_", &adamw_update, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"),
+          py::arg("exp_avg_sqs"), py::arg("step"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
+          py::arg("weight_decay"), py::arg("max_norm") = py::none(), py::arg("skip_nonfinite") = false,
+          py::arg("masters") = std::vector<OptT>{}, py::arg("row_masks") = std::vector<OptT>{});
 }

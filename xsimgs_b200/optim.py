@@ -1,0 +1,168 @@
+"""The end of a training step: gradient norm, clipping and the AdamW update
+over all leaves of a scene at once (csrc/optim.cu).
+
+The reference leaves the optimiser to its caller.  A caller of this package
+has the gradients of a handful of large leaves (means, quaternions, scales,
+opacities, SH coefficients) and of many small ones (camera poses), and these
+functions take them all in one or two launches, without a host round trip:
+
+  * `gradient_norm(grads)`: the global norm, and each tensor's if asked;
+  * `clip_gradients_(grads, max_norm)`: scales the gradients in place so that
+    their global norm is at most `max_norm`;
+  * `adamw_update_(params, grads, exp_avgs, exp_avg_sqs, step, ...)`: the
+    AdamW update, with the clipping coefficient applied on the way
+    (`max_norm`), rows that no sensor saw left as they are (`row_mask`) and
+    half-precision parameters kept beside 32-bit masters (`masters`);
+  * `AdamW`: a `torch.optim.Optimizer` over these.
+
+Tensors are float32, bfloat16 or float16 on one CUDA device; moments and
+masters are float32.  Work is enqueued on the current stream and nothing is
+read back.  Results do not depend on the run: sums are taken in a fixed order.
+"""
+from __future__ import annotations
+
+from collections.abc import Sequence
+
+import torch
+
+from ._native import _C
+
+
+def gradient_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0, per_tensor: bool = False):
+    """The norm of all elements of all `grads` as a 0-dim float32 tensor on
+    their device; `norm_type` is 2, 1 or inf.  `per_tensor`: also a tensor
+    with each one's norm.  Sums are held in 64 bits, so large and tiny
+    gradients neither overflow nor vanish on the way; NaN and infinite
+    elements show in the result.  A tensor with gaps or expanded dimensions is
+    copied first."""
+    return _C.gradient_norm(grads if isinstance(grads, list) else list(grads), norm_type, per_tensor)
+
+
+def clip_gradients_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
+    """Multiplies `grads` in place by min(1, max_norm / (norm + 1e-6)) and
+    returns the norm that they had.  An infinite norm gives the factor 0, a
+    NaN makes every gradient NaN.  The tensors must be dense and may not share
+    memory."""
+    return _C.clip_gradients_(grads if isinstance(grads, list) else list(grads), max_norm, norm_type)
+
+
+def adamw_step_counter(device, updates: int = 0) -> torch.Tensor:
+    """The `step` of `adamw_update_`: the number of updates taken, which the
+    call advances on the device, and a word that is zero between calls."""
+    return torch.tensor([updates, 0], dtype=torch.int64, device=device)
+
+
+def _values(v) -> list:
+    return [float(x) for x in v] if isinstance(v, (list, tuple)) else [float(v)]
+
+
+def adamw_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+                  exp_avg_sqs: Sequence[torch.Tensor], step: torch.Tensor, *, lr, betas=(0.9, 0.999), eps=1e-8,
+                  weight_decay=0.0, max_norm: float | None = None, skip_nonfinite: bool = False,
+                  masters: Sequence[torch.Tensor | None] | None = None,
+                  row_mask: torch.Tensor | Sequence[torch.Tensor | None] | None = None) -> torch.Tensor | None:
+    """One AdamW update of `params` in place, outside autograd.  With t the
+    number of updates taken so far plus one (`step`, from
+    `adamw_step_counter`):
+
+        m <- b1 m + (1 - b1) g,   v <- b2 v + (1 - b2) g^2,
+        w <- w - lr * weight_decay * w - lr * (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps)
+
+    lr, eps, weight_decay and both betas are one value for all tensors or a
+    list with one for each.  `max_norm`: g is the gradient clipped to that
+    global 2-norm (`grads` themselves stay as they are).  `skip_nonfinite`: a
+    norm that is NaN or infinite leaves parameters, moments and `step` as they
+    were.  With either, the norm before clipping is returned.  `masters`:
+    32-bit parameters that half-precision `params` are roundings of; both are
+    written.  `row_mask` (bool, one entry for each row of dimension 0; one for
+    all tensors or a list): rows with False keep parameter and moments.
+
+    Written tensors must be dense and may not share memory; moments and
+    masters have their parameter's sizes and order of dimensions.  A gradient
+    in another order is copied first.  Under graph capture the learning rate
+    is the one at capture."""
+    as_list = lambda v: v if isinstance(v, list) else list(v)  # noqa: E731
+    masks = [] if row_mask is None else [row_mask] if isinstance(row_mask, torch.Tensor) else list(row_mask)
+    return _C.adamw_update_(as_list(params), as_list(grads), as_list(exp_avgs), as_list(exp_avg_sqs), step,
+                            _values(lr), _values(betas[0]), _values(betas[1]), _values(eps), _values(weight_decay),
+                            max_norm, skip_nonfinite, [] if masters is None else as_list(masters), masks)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over `adamw_update_`: all parameter groups in one update.
+
+    Group options: lr, betas, eps, weight_decay.  `max_norm` clips the global
+    2-norm over all groups; `skip_nonfinite` passes over steps whose norm is
+    NaN or infinite.  Half-precision parameters get float32 masters.  The
+    number of updates is one counter on the device for all parameters, so a
+    parameter added later starts at the common count."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
+                 *, max_norm: float | None = None, skip_nonfinite: bool = False):
+        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
+            raise ValueError("AdamW: lr, eps and weight_decay must not be negative, betas in [0, 1)")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self.max_norm = max_norm
+        self.skip_nonfinite = skip_nonfinite
+        self._step: torch.Tensor | None = None
+
+    def _state(self, p: torch.Tensor) -> dict:
+        s = self.state[p]
+        if not s:
+            s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            s["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+            if p.dtype != torch.float32:
+                s["master"] = p.detach().to(torch.float32, copy=True)
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None, *, row_masks: dict | None = None) -> torch.Tensor | None:
+        """Updates every parameter that has a gradient; returns the global
+        gradient norm before clipping (None without `max_norm` and
+        `skip_nonfinite`).  `row_masks`: for a parameter, the rows to
+        update; the others keep their values and moments."""
+        if closure is not None:
+            with torch.enable_grad():
+                closure()
+        params, grads, ms, vs, masters, masks = [], [], [], [], [], []
+        lr, b1, b2, eps, decay = [], [], [], [], []
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                s = self._state(p)
+                params.append(p)
+                grads.append(p.grad)
+                ms.append(s["exp_avg"])
+                vs.append(s["exp_avg_sq"])
+                masters.append(s.get("master"))
+                masks.append(row_masks.get(p) if row_masks else None)
+                lr.append(group["lr"])
+                b1.append(group["betas"][0])
+                b2.append(group["betas"][1])
+                eps.append(group["eps"])
+                decay.append(group["weight_decay"])
+        if not params:
+            return None
+        if self._step is None:
+            self._step = adamw_step_counter(params[0].device)
+        return adamw_update_(params, grads, ms, vs, self._step, lr=lr, betas=(b1, b2), eps=eps, weight_decay=decay,
+                             max_norm=self.max_norm, skip_nonfinite=self.skip_nonfinite,
+                             masters=masters if any(m is not None for m in masters) else None,
+                             row_mask=masks if row_masks else None)
+
+    def state_dict(self) -> dict:
+        d = super().state_dict()
+        d["updates"] = 0 if self._step is None else int(self._step[0])
+        return d
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        super().load_state_dict({k: v for k, v in state_dict.items() if k != "updates"})
+        # the base class casts state to its parameter's type: masters and moments stay in 32 bits
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, mine):
+            for k, v in state_dict["state"].get(i, {}).items():
+                self.state[p][k] = v.to(device=p.device, dtype=torch.float32, copy=True)
+        device = mine[0].device
+        self._step = adamw_step_counter(device, int(state_dict.get("updates", 0)))
