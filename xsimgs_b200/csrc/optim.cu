@@ -48,18 +48,32 @@ __device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float x)
 }
 
 // ---------------------------------------------------------------- tables --
-// Tile k of a tensor holds its elements [k * tile, (k + 1) * tile); tensor t
-// of a table owns the tiles [first[t], first[t + 1]) of the launch.
+// A tensor is numbered from the 16-byte boundary at or below its first
+// element: its elements are the numbers [lead, end) from `base`, whatever its
+// offset, and every 16 bytes in between are one aligned vector.  Tile k holds
+// the numbers [k * tile, (k + 1) * tile); tensor t of a table owns the tiles
+// [first[t], first[t + 1]) of the launch.
 constexpr int kTileBytes = 16384;
 
 template <int N>
 struct SpanTable {
-    void* data[N];
-    int64_t n[N];
+    void* base[N];
+    int64_t end[N];
     int32_t first[N + 1];
+    uint8_t lead[N];
     uint8_t dtype[N];
     int32_t count;
 };
+
+// The part of tensor t in the tiles [tile, stop): numbers [lo, hi).
+struct Part {
+    int64_t lo, hi;
+};
+template <typename Table>
+__device__ __forceinline__ Part part_of(const Table& tab, int t, int32_t tile, int32_t stop) {
+    const int64_t per = kTileBytes / elem_size(tab.dtype[t]);
+    return {max(int64_t(tab.lead[t]), (tile - tab.first[t]) * per), min(tab.end[t], (stop - tab.first[t]) * per)};
+}
 
 // The run of tiles of block b out of `blocks`, and back.
 __host__ __device__ __forceinline__ int32_t run_start(int32_t tiles, int32_t blocks, int32_t b) {
@@ -96,6 +110,110 @@ template <int P>
 __device__ __forceinline__ double term(float x) {
     if constexpr (P == 2) return double(x) * double(x);
     return fabs(double(x));
+}
+
+__device__ __forceinline__ float2 halves(uint32_t u, int dtype) {
+    if (dtype == XSG_BF16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+}
+
+// Adds 16 elements, in `x` as 32 bits.  Their sum is first taken in 32 bits
+// (the conversions to 64 bits run at a quarter of the rate that a full-speed
+// read of 16-bit data needs), and goes on as it is unless squares may have
+// left the range in which 32 bits lose nothing: above 2^120, below 2^-96, or
+// not finite.  Zeros, which most entries of a sparse gradient are, end there.
+template <int P, int D>
+__device__ __forceinline__ void add16(double& acc, const float (&x)[16]) {
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i & 3] = P == 2 ? fmaf(x[i], x[i], s[i & 3]) : s[i & 3] + fabsf(x[i]);
+    const float sum = (s[0] + s[1]) + (s[2] + s[3]);
+    const bool safe = D == XSG_F16 || (P == 2 ? sum >= 0x1p-96f && sum <= 0x1p120f : sum <= 0x1p120f);
+    if (safe) {
+        acc += double(sum);
+        return;
+    }
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) any |= __float_as_uint(x[i]);
+    if ((any << 1) == 0) return;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc += term<P>(x[i]);
+}
+
+// Sum (or maximum) over the numbers [lo, hi) of a tensor, by the block.
+template <int P, int D>
+__device__ __forceinline__ double reduce_part(const void* base, Part part) {
+    constexpr int V = 16 / elem_size(D);  // elements of a vector
+    constexpr int kUnroll = 4;
+    const auto* vec = static_cast<const uint4*>(base);
+    const int64_t first = (part.lo + V - 1) / V, last = part.hi / V;  // whole vectors
+    double acc = 0.0;
+    [[maybe_unused]] uint32_t top = 0;  // of |x|'s bits: NaN > inf > numbers
+    const auto take = [&](const uint4 (&q)[kUnroll]) {
+        if constexpr (P == kNormInf) {
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (D == XSG_F32) top = max(top, w[i] & 0x7fffffffu);
+                    else top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+                }
+            }
+        } else if constexpr (D == XSG_F32) {
+            float x[16];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                x[4 * k] = __uint_as_float(q[k].x), x[4 * k + 1] = __uint_as_float(q[k].y);
+                x[4 * k + 2] = __uint_as_float(q[k].z), x[4 * k + 3] = __uint_as_float(q[k].w);
+            }
+            add16<P, D>(acc, x);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kUnroll; k += 2) {
+                float x[16];
+                const uint32_t w[8] = {q[k].x, q[k].y, q[k].z, q[k].w, q[k + 1].x, q[k + 1].y, q[k + 1].z, q[k + 1].w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = halves(w[i], D);
+                    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+                }
+                add16<P, D>(acc, x);
+            }
+        }
+    };
+    int64_t i = first + threadIdx.x;
+    for (; i + (kUnroll - 1) * kOptThreads < last; i += kUnroll * kOptThreads) {
+        uint4 q[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) q[k] = __ldg(vec + i + k * kOptThreads);
+        take(q);
+    }
+    if (i < last) {
+        uint4 q[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+            q[k] = i + k * kOptThreads < last ? __ldg(vec + i + k * kOptThreads) : make_uint4(0, 0, 0, 0);
+        take(q);
+    }
+    if constexpr (P == kNormInf) {
+        const uint32_t one = D == XSG_F32 ? top : max(top & 0xffffu, top >> 16);
+        acc = double(D == XSG_F32 ? __uint_as_float(one) : halves(one, D).x);
+    }
+    // the elements before the first and after the last whole vector
+    const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
+    const int64_t odd = threadIdx.x < V ? part.lo + threadIdx.x : tail + threadIdx.x - V;
+    if (threadIdx.x < 2 * V && odd < (threadIdx.x < V ? head : part.hi))
+        acc = join<P>(acc, term<P>(load_as(base, D, odd)));
+    return acc;
+}
+
+template <int P>
+__device__ __forceinline__ double reduce_part(const void* base, int dtype, Part part) {
+    if (dtype == XSG_F32) return reduce_part<P, XSG_F32>(base, part);
+    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16>(base, part);
+    return reduce_part<P, XSG_F16>(base, part);
 }
 
 // Over the block, in a fixed order; every thread gets the result.  `smem`
@@ -139,13 +257,7 @@ __global__ void __launch_bounds__(kOptThreads)
     for (int t = owner_of(tab, tile); tile < end; ++t) {
         const int32_t stop = min(end, tab.first[t + 1]);
         if (stop <= tile) continue;
-        const int dtype = tab.dtype[t];
-        const int64_t per = kTileBytes / elem_size(dtype);
-        const int64_t lo = (tile - tab.first[t]) * per;
-        const int64_t hi = min(tab.n[t], int64_t(stop - tab.first[t]) * per);
-        double acc = 0.0;
-        for (int64_t i = lo + threadIdx.x; i < hi; i += kOptThreads)
-            acc = join<P>(acc, term<P>(load_as(tab.data[t], dtype, i)));
+        double acc = reduce_part<P>(tab.base[t], tab.dtype[t], part_of(tab, t, tile, stop));
         if (slots) {
             acc = block_reduce<P>(acc, smem);
             if (threadIdx.x == 0) slots[blockIdx.x + t] = acc;
@@ -212,11 +324,9 @@ __global__ void __launch_bounds__(kOptThreads)
         const int32_t stop = min(end, tab.first[t + 1]);
         if (stop <= tile) continue;
         const int dtype = tab.dtype[t];
-        const int64_t per = kTileBytes / elem_size(dtype);
-        const int64_t lo = (tile - tab.first[t]) * per;
-        const int64_t hi = min(tab.n[t], int64_t(stop - tab.first[t]) * per);
-        for (int64_t i = lo + threadIdx.x; i < hi; i += kOptThreads)
-            store_as(tab.data[t], dtype, i, load_as(tab.data[t], dtype, i) * c);
+        const Part part = part_of(tab, t, tile, stop);
+        for (int64_t i = part.lo + threadIdx.x; i < part.hi; i += kOptThreads)
+            store_as(tab.base[t], dtype, i, load_as(tab.base[t], dtype, i) * c);
         tile = stop;
     }
 }
@@ -355,11 +465,14 @@ std::vector<SpanLaunch> plan_spans(const xsg_span* spans, int64_t n) {
         for (int t = 0; t < L.tab.count; ++t) {
             const xsg_span& s = spans[L.first_span + t];
             const int64_t per = kTileBytes / elem_size(s.dtype);
-            L.tab.data[t] = s.data;
-            L.tab.n[t] = s.n;
+            const auto at = reinterpret_cast<uintptr_t>(s.data);
+            const int64_t lead = int64_t(at % 16) / elem_size(s.dtype);
+            L.tab.base[t] = reinterpret_cast<void*>(at - at % 16);
+            L.tab.lead[t] = uint8_t(lead);
+            L.tab.end[t] = lead + s.n;
             L.tab.dtype[t] = uint8_t(s.dtype);
             L.tab.first[t] = int32_t(tiles);
-            tiles += (s.n + per - 1) / per;
+            tiles += s.n ? (lead + s.n + per - 1) / per : 0;
         }
         L.tab.first[L.tab.count] = int32_t(tiles);
         L.blocks = int(std::max<int64_t>(1, std::min<int64_t>(tiles, kOptBlocks)));
