@@ -28,7 +28,8 @@ namespace xsg {
 namespace {
 
 constexpr int kOptThreads = 256;
-constexpr int kOptBlocks = 148 * 4;      // blocks a launch at most
+constexpr int kOptResident = 4;          // blocks an SM
+constexpr int kOptBlocks = 148 * kOptResident;  // blocks a launch at most: all of them run at once
 constexpr float kClipEps = 1e-6f;
 constexpr int kNormInf = 0;
 
@@ -146,8 +147,9 @@ template <int P, int D>
 __device__ __forceinline__ double reduce_part(const void* base, Part part) {
     constexpr int V = 16 / elem_size(D);  // elements of a vector
     constexpr int kUnroll = 4;
-    const auto* vec = static_cast<const uint4*>(base);
     const int64_t first = (part.lo + V - 1) / V, last = part.hi / V;  // whole vectors
+    const uint4* vec = static_cast<const uint4*>(base) + first;
+    const int n = int(max(last - first, int64_t(0)));  // a block's part is below 2^31 vectors
     double acc = 0.0;
     [[maybe_unused]] uint32_t top = 0;  // of |x|'s bits: NaN > inf > numbers
     const auto take = [&](const uint4 (&q)[kUnroll]) {
@@ -183,18 +185,18 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part) {
             }
         }
     };
-    int64_t i = first + threadIdx.x;
-    for (; i + (kUnroll - 1) * kOptThreads < last; i += kUnroll * kOptThreads) {
+    int i = threadIdx.x;
+    for (; i + (kUnroll - 1) * kOptThreads < n; i += kUnroll * kOptThreads) {
         uint4 q[kUnroll];
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k) q[k] = __ldg(vec + i + k * kOptThreads);
         take(q);
     }
-    if (i < last) {
+    if (i < n) {
         uint4 q[kUnroll];
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k)
-            q[k] = i + k * kOptThreads < last ? __ldg(vec + i + k * kOptThreads) : make_uint4(0, 0, 0, 0);
+            q[k] = i + k * kOptThreads < n ? __ldg(vec + i + k * kOptThreads) : make_uint4(0, 0, 0, 0);
         take(q);
     }
     if constexpr (P == kNormInf) {
@@ -246,7 +248,7 @@ __device__ __forceinline__ float clip_coefficient(float norm, float max_norm) {
 // each tensor's norm is asked for, slots[b + t] for its part of tensor t
 // (b + t grows along the runs, so that no two parts share a slot).
 template <int P, int N>
-__global__ void __launch_bounds__(kOptThreads)
+__global__ void __launch_bounds__(kOptThreads, kOptResident)
     norm_partial_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums,
                         double* __restrict__ slots) {
     __shared__ double smem[33];
@@ -306,10 +308,55 @@ __global__ void __launch_bounds__(kOptThreads)
     if (lane == 0) norms[t] = root<P>(v);
 }
 
-// g <- c g.  The product is taken in 32 bits and rounded once to g's type;
-// c = 1 leaves the data alone.
+// g <- c g over the numbers [lo, hi) of a tensor, by the block, from the end
+// to the start.  The product is taken in 32 bits and rounded once to g's type.
+template <int D>
+__device__ __forceinline__ uint32_t scaled(uint32_t w, float c) {
+    if constexpr (D == XSG_F32) return __float_as_uint(__uint_as_float(w) * c);
+    const float2 f = halves(w, D);
+    uint32_t r;
+    if constexpr (D == XSG_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f.x * c, f.y * c);
+        memcpy(&r, &h, 4);
+    } else {
+        const __half2 h = __floats2half2_rn(f.x * c, f.y * c);
+        memcpy(&r, &h, 4);
+    }
+    return r;
+}
+
+template <int D>
+__device__ __forceinline__ void scale_part(void* base, Part part, float c) {
+    constexpr int V = 16 / elem_size(D);
+    constexpr int kUnroll = 4, kStep = kUnroll * kOptThreads;
+    const int64_t first = (part.lo + V - 1) / V, last = part.hi / V;
+    uint4* vec = static_cast<uint4*>(base) + first;
+    const int n = int(max(last - first, int64_t(0)));  // a block's part is below 2^31 vectors
+    int i = n / kStep * kStep + threadIdx.x;
+    for (int j = i; j < n; j += kOptThreads) {
+        const uint4 q = vec[j];
+        vec[j] = make_uint4(scaled<D>(q.x, c), scaled<D>(q.y, c), scaled<D>(q.z, c), scaled<D>(q.w, c));
+    }
+    for (i -= kStep; i >= 0; i -= kStep) {
+        uint4 q[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) q[k] = vec[i + k * kOptThreads];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k)
+            vec[i + k * kOptThreads] =
+                make_uint4(scaled<D>(q[k].x, c), scaled<D>(q[k].y, c), scaled<D>(q[k].z, c), scaled<D>(q[k].w, c));
+    }
+    const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
+    const int64_t odd = threadIdx.x < V ? part.lo + threadIdx.x : tail + threadIdx.x - V;
+    if (threadIdx.x < 2 * V && odd < (threadIdx.x < V ? head : part.hi))
+        store_as(base, D, odd, load_as(base, D, odd) * c);
+}
+
+// The second pass of clipping.  c = 1 leaves the data alone.  Every block
+// takes the run that it had in the first pass, backwards, so that what the
+// first pass read last, and the L2 still holds, comes first.
 template <int P, int N>
-__global__ void __launch_bounds__(kOptThreads)
+__global__ void __launch_bounds__(kOptThreads, kOptResident)
     clip_scale_kernel(const __grid_constant__ SpanTable<N> tab, const double* __restrict__ sums, int n_sums,
                       float max_norm, float* __restrict__ norm) {
     __shared__ double smem[33];
@@ -318,21 +365,23 @@ __global__ void __launch_bounds__(kOptThreads)
     const float c = clip_coefficient(total, max_norm);
     if (c == 1.f) return;
     const int32_t tiles = tab.first[tab.count];
-    int32_t tile = run_start(tiles, gridDim.x, blockIdx.x);
-    const int32_t end = run_start(tiles, gridDim.x, blockIdx.x + 1);
-    for (int t = owner_of(tab, tile); tile < end; ++t) {
-        const int32_t stop = min(end, tab.first[t + 1]);
-        if (stop <= tile) continue;
-        const int dtype = tab.dtype[t];
+    const int32_t begin = run_start(tiles, gridDim.x, blockIdx.x);
+    int32_t stop = run_start(tiles, gridDim.x, blockIdx.x + 1);
+    for (int t = owner_of(tab, stop - 1); stop > begin; --t) {
+        const int32_t tile = max(begin, tab.first[t]);
+        if (tile >= stop) continue;
         const Part part = part_of(tab, t, tile, stop);
-        for (int64_t i = part.lo + threadIdx.x; i < part.hi; i += kOptThreads)
-            store_as(tab.base[t], dtype, i, load_as(tab.base[t], dtype, i) * c);
-        tile = stop;
+        const int dtype = tab.dtype[t];
+        if (dtype == XSG_F32) scale_part<XSG_F32>(tab.base[t], part, c);
+        else if (dtype == XSG_BF16) scale_part<XSG_BF16>(tab.base[t], part, c);
+        else scale_part<XSG_F16>(tab.base[t], part, c);
+        stop = tile;
     }
 }
 
 // ----------------------------------------------------------------- AdamW --
 constexpr int kAdamTile = 2048;  // elements
+constexpr int kAdamResident = 3;  // blocks an SM
 constexpr int kAdamGroups = 32;
 
 struct AdamHyper {
@@ -340,22 +389,28 @@ struct AdamHyper {
     float log_beta1, log_beta2;
 };
 
+// Elements are numbered from `lead` on, as above, in vectors of four; the
+// pointers are those of number 0.  All arrays of a tensor have to have the
+// same lead for that (`vec`); where they do not, lead is 0 and elements go
+// one by one.
+struct AdamEntry {
+    void* param;
+    const void* grad;
+    float* exp_avg;
+    float* exp_avg_sq;
+    float* master;
+    const uint8_t* rows;
+    int64_t end;
+    int32_t row_size;
+    uint8_t lead, vec, group, param_dtype, grad_dtype;
+};
+
 template <int N>
 struct AdamTable {
-    void* param[N];
-    const void* grad[N];
-    float* exp_avg[N];
-    float* exp_avg_sq[N];
-    float* master[N];
-    const uint8_t* rows[N];
-    int64_t n[N];
-    int64_t row_size[N];
+    AdamEntry entry[N];
     int32_t first[N + 1];
-    uint8_t param_dtype[N];
-    uint8_t grad_dtype[N];
-    uint8_t group[N];
-    AdamHyper hyper[kAdamGroups];
     int32_t count;
+    AdamHyper hyper[kAdamGroups];
 };
 
 struct AdamCall {
@@ -369,16 +424,144 @@ struct AdamCall {
     float* norm;
 };
 
-template <int N>
-__global__ void __launch_bounds__(kOptThreads)
+struct AdamScale {
+    float c, beta1, rest1, beta2, rest2, lr_decay, eps, step_size, root_scale;
+};
+
+__device__ __forceinline__ void adam_element(const AdamScale& h, float g, float& m, float& v, float& w) {
+    g *= h.c;
+    m = fmaf(h.beta1, m, h.rest1 * g);
+    v = fmaf(h.beta2, v, h.rest2 * g * g);
+    w = fmaf(-h.lr_decay, w, w);
+    w -= h.step_size * m / fmaf(sqrtf(v), h.root_scale, h.eps);
+}
+
+__device__ __forceinline__ void load4(float (&x)[4], const void* p, int dtype, int64_t i) {
+    if (dtype == XSG_F32) {
+        const float4 q = static_cast<const float4*>(p)[i];
+        x[0] = q.x, x[1] = q.y, x[2] = q.z, x[3] = q.w;
+    } else {
+        const uint2 q = static_cast<const uint2*>(p)[i];
+        const float2 a = halves(q.x, dtype), b = halves(q.y, dtype);
+        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    }
+}
+
+__device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const float (&x)[4]) {
+    if (dtype == XSG_F32) {
+        static_cast<float4*>(p)[i] = make_float4(x[0], x[1], x[2], x[3]);
+    } else if (dtype == XSG_BF16) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+        uint2 q;
+        memcpy(&q.x, &a, 4);
+        memcpy(&q.y, &b, 4);
+        static_cast<uint2*>(p)[i] = q;
+    } else {
+        const __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
+        uint2 q;
+        memcpy(&q.x, &a, 4);
+        memcpy(&q.y, &b, 4);
+        static_cast<uint2*>(p)[i] = q;
+    }
+}
+
+// The update over the numbers [lo, hi) of a tensor, by the block.  kF32: all
+// arrays are in 32 bits and there is no master, so no branch on the types
+// stands between the loads.
+template <bool kF32>
+__device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const AdamScale& h) {
+    constexpr int kUnroll = 2;
+    const int pd = kF32 ? XSG_F32 : e.param_dtype, gd = kF32 ? XSG_F32 : e.grad_dtype;
+    float* master = kF32 ? nullptr : e.master;
+    // rows: of the part's first element by one 64-bit division, of the others
+    // by a 32-bit one of their distance (part < 2^31, row_size < 2^30)
+    const int64_t origin = part.lo - e.lead;
+    const uint32_t rs = e.rows ? uint32_t(e.row_size) : 1u;
+    const int64_t row0 = e.rows ? origin / rs : 0;
+    const uint32_t rem0 = e.rows ? uint32_t(origin - row0 * rs) : 0u;
+    const auto one = [&](int64_t i) {
+        if (e.rows && !e.rows[row0 + (rem0 + uint32_t(i - part.lo)) / rs]) return;
+        float m = e.exp_avg[i], v = e.exp_avg_sq[i];
+        float w = master ? master[i] : load_as(e.param, pd, i);
+        adam_element(h, load_as(e.grad, gd, i), m, v, w);
+        e.exp_avg[i] = m;
+        e.exp_avg_sq[i] = v;
+        if (master) master[i] = w;
+        store_as(e.param, pd, i, w);
+    };
+    if (!e.vec) {
+        for (int64_t i = part.lo + threadIdx.x; i < part.hi; i += kOptThreads) one(i);
+        return;
+    }
+    const int64_t first = (part.lo + 3) / 4, last = part.hi / 4;
+    const int n = int(max(last - first, int64_t(0)));
+    const uint32_t skew = rem0 + uint32_t(4 * first - part.lo);  // of vector 0 from the row's start
+    for (int at = threadIdx.x; at < n; at += kUnroll * kOptThreads) {
+        float w[kUnroll][4], g[kUnroll][4], m[kUnroll][4], v[kUnroll][4];
+        uint32_t keep[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            keep[k] = at + k * kOptThreads < n ? 15u : 0u;
+            if (e.rows && keep[k]) {
+                const uint32_t x = skew + 4u * uint32_t(at + k * kOptThreads), r = x / rs, rem = x - r * rs;
+                const uint8_t* row = e.rows + row0 + r;
+                keep[k] = row[0] ? 1u : 0u;
+#pragma unroll
+                for (uint32_t j = 1; j < 4; ++j) {
+                    // element j's row: at most j rows on
+                    const uint32_t y = rem + j, on = (y >= rs) + (j >= 2 && y >= 2 * rs) + (j >= 3 && y >= 3 * rs);
+                    keep[k] |= row[on] ? 1u << j : 0u;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const int64_t i = first + at + k * kOptThreads;
+            if (!keep[k]) continue;
+            load4(g[k], e.grad, gd, i);
+            load4(m[k], e.exp_avg, XSG_F32, i);
+            load4(v[k], e.exp_avg_sq, XSG_F32, i);
+            if (master) load4(w[k], master, XSG_F32, i);
+            else load4(w[k], e.param, pd, i);
+        }
+#pragma unroll
+        for (int k = 0; k < kUnroll; ++k) {
+            const int64_t i = first + at + k * kOptThreads;
+            if (!keep[k]) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float nm = m[k][j], nv = v[k][j], nw = w[k][j];
+                adam_element(h, g[k][j], nm, nv, nw);
+                if (keep[k] >> j & 1) m[k][j] = nm, v[k][j] = nv, w[k][j] = nw;
+            }
+            store4(e.exp_avg, XSG_F32, i, m[k]);
+            store4(e.exp_avg_sq, XSG_F32, i, v[k]);
+            if (master) store4(master, XSG_F32, i, w[k]);
+            if (keep[k] == 15u || (!master && pd == XSG_F32)) {
+                store4(e.param, pd, i, w[k]);
+            } else {
+                // a row that is passed over keeps its parameter's bits, whatever its master says
+                for (int j = 0; j < 4; ++j)
+                    if (keep[k] >> j & 1) store_as(e.param, pd, 4 * i + j, w[k][j]);
+            }
+        }
+    }
+    const int64_t head = min(first * 4, part.hi), tail = max(last * 4, head);
+    const int64_t odd = threadIdx.x < 4 ? part.lo + threadIdx.x : tail + threadIdx.x - 4;
+    if (threadIdx.x < 8 && odd < (threadIdx.x < 4 ? head : part.hi)) one(odd);
+}
+
+template <int N, bool kF32>
+__global__ void __launch_bounds__(kOptThreads, kAdamResident)
     adamw_kernel(const __grid_constant__ AdamTable<N> tab, const __grid_constant__ AdamCall call) {
     __shared__ double smem[33];
-    float c = 1.f;
+    AdamScale h;
+    h.c = 1.f;
     if (call.sums) {
         const float total = total_norm<2>(call.sums, call.n_sums, smem);
         if (blockIdx.x == 0 && threadIdx.x == 0 && call.norm) *call.norm = total;
         if (call.skip_nonfinite && !isfinite(total)) return;  // every block alike: nothing changes
-        if (call.clip) c = clip_coefficient(total, call.max_norm);
+        if (call.clip) h.c = clip_coefficient(total, call.max_norm);
     }
     const float steps = float(call.step[0] + 1);
     const int32_t tiles = tab.first[tab.count];
@@ -387,25 +570,15 @@ __global__ void __launch_bounds__(kOptThreads)
     for (int t = owner_of(tab, tile); tile < end; ++t) {
         const int32_t stop = min(end, tab.first[t + 1]);
         if (stop <= tile) continue;
-        const AdamHyper h = tab.hyper[tab.group[t]];
+        const AdamEntry& e = tab.entry[t];
+        const AdamHyper& y = tab.hyper[e.group];
+        h.beta1 = y.beta1, h.rest1 = y.rest1, h.beta2 = y.beta2, h.rest2 = y.rest2;
+        h.lr_decay = y.lr_decay, h.eps = y.eps;
         // 1 - b^t without the cancellation of 1 - pow(b, t)
-        const float step_size = h.lr / -expm1f(steps * h.log_beta1);
-        const float scale2 = rsqrtf(-expm1f(steps * h.log_beta2));
-        const int64_t lo = int64_t(tile - tab.first[t]) * kAdamTile;
-        const int64_t hi = min(tab.n[t], int64_t(stop - tab.first[t]) * kAdamTile);
-        for (int64_t i = lo + threadIdx.x; i < hi; i += kOptThreads) {
-            if (tab.rows[t] && !tab.rows[t][i / tab.row_size[t]]) continue;
-            const float g = load_as(tab.grad[t], tab.grad_dtype[t], i) * c;
-            const float m = fmaf(h.beta1, tab.exp_avg[t][i], h.rest1 * g);
-            const float v = fmaf(h.beta2, tab.exp_avg_sq[t][i], h.rest2 * g * g);
-            float w = tab.master[t] ? tab.master[t][i] : load_as(tab.param[t], tab.param_dtype[t], i);
-            w = fmaf(-h.lr_decay, w, w);
-            w -= step_size * m / fmaf(sqrtf(v), scale2, h.eps);
-            tab.exp_avg[t][i] = m;
-            tab.exp_avg_sq[t][i] = v;
-            if (tab.master[t]) tab.master[t][i] = w;
-            store_as(tab.param[t], tab.param_dtype[t], i, w);
-        }
+        h.step_size = y.lr / -expm1f(steps * y.log_beta1);
+        h.root_scale = rsqrtf(-expm1f(steps * y.log_beta2));
+        adam_part<kF32>(e, {max(int64_t(e.lead), int64_t(tile - tab.first[t]) * kAdamTile),
+                            min(e.end, int64_t(stop - tab.first[t]) * kAdamTile)}, h);
         tile = stop;
     }
     if (call.advance) {
@@ -423,7 +596,7 @@ __global__ void __launch_bounds__(kOptThreads)
 
 // ------------------------------------------------------------------ host --
 constexpr int kSpans = 1024;
-constexpr int kAdamSpans = 320;
+constexpr int kAdamSpans = 400;
 static_assert(sizeof(SpanTable<kSpans>) <= 32000 && sizeof(AdamTable<kAdamSpans>) <= 32000,
               "kernel parameters hold 32764 bytes");
 
@@ -451,6 +624,21 @@ int check_spans(const xsg_span* spans, int64_t n, const char* what) {
                     std::string(what) + ": misaligned pointer");
     }
     return XSG_OK;
+}
+
+// The element that the arrays of an update have in common as their first past
+// a vector's boundary, or -1 if they have none.
+int common_lead(const xsg_adamw_span& s) {
+    int lead = -1;
+    const auto same = [&](const void* p, int size) {
+        const int l = int(reinterpret_cast<uintptr_t>(p) / size % 4);
+        const bool ok = lead < 0 || l == lead;
+        lead = l;
+        return ok;
+    };
+    const bool all = same(s.param, elem_size(s.param_dtype)) && same(s.grad, elem_size(s.grad_dtype)) &&
+                     same(s.exp_avg, 4) && same(s.exp_avg_sq, 4) && (!s.master || same(s.master, 4));
+    return all ? lead : -1;
 }
 
 // Cuts the spans into launches of at most kSpans tensors.
@@ -593,7 +781,8 @@ static int adamw_update(const xsg_adamw_span* spans_host, int64_t n_spans, int64
         XSG_REQUIRE(s.n >= 0 && s.n < kMaxElems - total, "adamw_update: bad element count");
         total += s.n;
         XSG_REQUIRE(s.n == 0 || (s.param && s.grad && s.exp_avg && s.exp_avg_sq), "adamw_update: null pointer");
-        XSG_REQUIRE(!s.row_mask || s.row_size > 0, "adamw_update: a row mask needs a row size");
+        XSG_REQUIRE(!s.row_mask || (s.row_size > 0 && s.row_size < (int64_t(1) << 30)),
+                    "adamw_update: a row mask needs a row size below 2^30");
         const auto off = [](const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
         XSG_REQUIRE(!off(s.param, elem_size(s.param_dtype)) && !off(s.grad, elem_size(s.grad_dtype)) &&
                         !off(s.exp_avg, 4) && !off(s.exp_avg_sq, 4) && !off(s.master, 4),
@@ -621,6 +810,7 @@ static int adamw_update(const xsg_adamw_span* spans_host, int64_t n_spans, int64
     for (int64_t i = 0; i < n_spans;) {
         int64_t tiles = 0;
         int groups = 0, t = 0;
+        bool f32 = true;
         for (; t < kAdamSpans && i < n_spans; ++t, ++i) {
             const xsg_adamw_span& s = spans_host[i];
             AdamHyper h{};
@@ -637,27 +827,34 @@ static int adamw_update(const xsg_adamw_span* spans_host, int64_t n_spans, int64
             while (g < groups && std::memcmp(&tab.hyper[g], &h, sizeof(h)) != 0) ++g;
             if (g == kAdamGroups) break;
             if (g == groups) tab.hyper[groups++] = h;
-            tab.group[t] = uint8_t(g);
-            tab.param[t] = s.param;
-            tab.grad[t] = s.grad;
-            tab.exp_avg[t] = s.exp_avg;
-            tab.exp_avg_sq[t] = s.exp_avg_sq;
-            tab.master[t] = s.master;
-            tab.rows[t] = s.row_mask;
-            tab.n[t] = s.n;
-            tab.row_size[t] = s.row_size;
-            tab.param_dtype[t] = uint8_t(s.param_dtype);
-            tab.grad_dtype[t] = uint8_t(s.grad_dtype);
+            AdamEntry& e = tab.entry[t];
+            const int lead = common_lead(s);
+            const auto back = [&](void* p, int size) { return static_cast<char*>(p) - std::max(lead, 0) * size; };
+            e.vec = lead >= 0;
+            e.lead = uint8_t(std::max(lead, 0));
+            e.group = uint8_t(g);
+            e.param = back(s.param, elem_size(s.param_dtype));
+            e.grad = back(const_cast<void*>(s.grad), elem_size(s.grad_dtype));
+            e.exp_avg = reinterpret_cast<float*>(back(s.exp_avg, 4));
+            e.exp_avg_sq = reinterpret_cast<float*>(back(s.exp_avg_sq, 4));
+            e.master = s.master ? reinterpret_cast<float*>(back(s.master, 4)) : nullptr;
+            e.rows = s.row_mask;
+            e.end = e.lead + s.n;
+            e.row_size = int32_t(s.row_size);
+            e.param_dtype = uint8_t(s.param_dtype);
+            e.grad_dtype = uint8_t(s.grad_dtype);
+            f32 = f32 && s.param_dtype == XSG_F32 && s.grad_dtype == XSG_F32 && !s.master;
             tab.first[t] = int32_t(tiles);
-            tiles += (s.n + kAdamTile - 1) / kAdamTile;
+            tiles += s.n ? (e.lead + s.n + kAdamTile - 1) / kAdamTile : 0;
         }
         tab.first[t] = int32_t(tiles);
         tab.count = t;
         const bool last = i >= n_spans;
         call.advance = last;
         call.norm = last ? norm : nullptr;
-        const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>(tiles, kOptBlocks)));
-        launch(adamw_kernel<kAdamSpans>, blocks, kOptThreads, 0, as_cuda(stream), tab, call);
+        const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>(tiles, 148 * kAdamResident)));
+        launch(f32 ? adamw_kernel<kAdamSpans, true> : adamw_kernel<kAdamSpans, false>, blocks, kOptThreads, 0,
+               as_cuda(stream), tab, call);
     }
     return check_launch("adamw_update");
 }
