@@ -380,8 +380,8 @@ __global__ void __launch_bounds__(kOptThreads, kOptResident)
 }
 
 // ----------------------------------------------------------------- AdamW --
-constexpr int kAdamTile = 2048;  // elements
-constexpr int kAdamResident = 3;  // blocks an SM
+constexpr int kAdamTile = 4096;  // elements
+constexpr int kAdamResident = 4;  // blocks an SM
 constexpr int kAdamGroups = 32;
 
 struct AdamHyper {
@@ -470,7 +470,6 @@ __device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const floa
 // stands between the loads.
 template <bool kF32>
 __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const AdamScale& h) {
-    constexpr int kUnroll = 2;
     const int pd = kF32 ? XSG_F32 : e.param_dtype, gd = kF32 ? XSG_F32 : e.grad_dtype;
     float* master = kF32 ? nullptr : e.master;
     // rows: of the part's first element by one 64-bit division, of the others
@@ -496,54 +495,42 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
     const int64_t first = (part.lo + 3) / 4, last = part.hi / 4;
     const int n = int(max(last - first, int64_t(0)));
     const uint32_t skew = rem0 + uint32_t(4 * first - part.lo);  // of vector 0 from the row's start
-    for (int at = threadIdx.x; at < n; at += kUnroll * kOptThreads) {
-        float w[kUnroll][4], g[kUnroll][4], m[kUnroll][4], v[kUnroll][4];
-        uint32_t keep[kUnroll];
+    for (int at = threadIdx.x; at < n; at += kOptThreads) {
+        uint32_t keep = 15u;
+        if (e.rows) {
+            const uint32_t x = skew + 4u * uint32_t(at), r = x / rs, rem = x - r * rs;
+            const uint8_t* row = e.rows + row0 + r;
+            keep = row[0] ? 1u : 0u;
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            keep[k] = at + k * kOptThreads < n ? 15u : 0u;
-            if (e.rows && keep[k]) {
-                const uint32_t x = skew + 4u * uint32_t(at + k * kOptThreads), r = x / rs, rem = x - r * rs;
-                const uint8_t* row = e.rows + row0 + r;
-                keep[k] = row[0] ? 1u : 0u;
-#pragma unroll
-                for (uint32_t j = 1; j < 4; ++j) {
-                    // element j's row: at most j rows on
-                    const uint32_t y = rem + j, on = (y >= rs) + (j >= 2 && y >= 2 * rs) + (j >= 3 && y >= 3 * rs);
-                    keep[k] |= row[on] ? 1u << j : 0u;
-                }
+            for (uint32_t j = 1; j < 4; ++j) {
+                // element j's row: at most j rows on
+                const uint32_t y = rem + j, on = (y >= rs) + (j >= 2 && y >= 2 * rs) + (j >= 3 && y >= 3 * rs);
+                keep |= row[on] ? 1u << j : 0u;
             }
+            if (!keep) continue;
         }
+        const int64_t i = first + at;
+        float w[4], g[4], m[4], v[4];
+        load4(g, e.grad, gd, i);
+        load4(m, e.exp_avg, XSG_F32, i);
+        load4(v, e.exp_avg_sq, XSG_F32, i);
+        if (master) load4(w, master, XSG_F32, i);
+        else load4(w, e.param, pd, i);
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            const int64_t i = first + at + k * kOptThreads;
-            if (!keep[k]) continue;
-            load4(g[k], e.grad, gd, i);
-            load4(m[k], e.exp_avg, XSG_F32, i);
-            load4(v[k], e.exp_avg_sq, XSG_F32, i);
-            if (master) load4(w[k], master, XSG_F32, i);
-            else load4(w[k], e.param, pd, i);
+        for (int j = 0; j < 4; ++j) {
+            float nm = m[j], nv = v[j], nw = w[j];
+            adam_element(h, g[j], nm, nv, nw);
+            if (keep >> j & 1) m[j] = nm, v[j] = nv, w[j] = nw;
         }
-#pragma unroll
-        for (int k = 0; k < kUnroll; ++k) {
-            const int64_t i = first + at + k * kOptThreads;
-            if (!keep[k]) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float nm = m[k][j], nv = v[k][j], nw = w[k][j];
-                adam_element(h, g[k][j], nm, nv, nw);
-                if (keep[k] >> j & 1) m[k][j] = nm, v[k][j] = nv, w[k][j] = nw;
-            }
-            store4(e.exp_avg, XSG_F32, i, m[k]);
-            store4(e.exp_avg_sq, XSG_F32, i, v[k]);
-            if (master) store4(master, XSG_F32, i, w[k]);
-            if (keep[k] == 15u || (!master && pd == XSG_F32)) {
-                store4(e.param, pd, i, w[k]);
-            } else {
-                // a row that is passed over keeps its parameter's bits, whatever its master says
-                for (int j = 0; j < 4; ++j)
-                    if (keep[k] >> j & 1) store_as(e.param, pd, 4 * i + j, w[k][j]);
-            }
+        store4(e.exp_avg, XSG_F32, i, m);
+        store4(e.exp_avg_sq, XSG_F32, i, v);
+        if (master) store4(master, XSG_F32, i, w);
+        if (keep == 15u || (!master && pd == XSG_F32)) {
+            store4(e.param, pd, i, w);
+        } else {
+            // a row that is passed over keeps its parameter's bits, whatever its master says
+            for (int j = 0; j < 4; ++j)
+                if (keep >> j & 1) store_as(e.param, pd, 4 * i + j, w[j]);
         }
     }
     const int64_t head = min(first * 4, part.hi), tail = max(last * 4, head);
@@ -564,22 +551,23 @@ __global__ void __launch_bounds__(kOptThreads, kAdamResident)
         if (call.clip) h.c = clip_coefficient(total, call.max_norm);
     }
     const float steps = float(call.step[0] + 1);
+    // tiles in turn: a part of a masked tensor may have little to do
     const int32_t tiles = tab.first[tab.count];
-    int32_t tile = run_start(tiles, gridDim.x, blockIdx.x);
-    const int32_t end = run_start(tiles, gridDim.x, blockIdx.x + 1);
-    for (int t = owner_of(tab, tile); tile < end; ++t) {
-        const int32_t stop = min(end, tab.first[t + 1]);
-        if (stop <= tile) continue;
+    int t = -1;
+    for (int32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        if (t < 0 || tile >= tab.first[t + 1]) {
+            if (t < 0) t = owner_of(tab, tile);
+            while (tile >= tab.first[t + 1]) ++t;
+            const AdamHyper& y = tab.hyper[tab.entry[t].group];
+            h.beta1 = y.beta1, h.rest1 = y.rest1, h.beta2 = y.beta2, h.rest2 = y.rest2;
+            h.lr_decay = y.lr_decay, h.eps = y.eps;
+            // 1 - b^t without the cancellation of 1 - pow(b, t)
+            h.step_size = y.lr / -expm1f(steps * y.log_beta1);
+            h.root_scale = rsqrtf(-expm1f(steps * y.log_beta2));
+        }
         const AdamEntry& e = tab.entry[t];
-        const AdamHyper& y = tab.hyper[e.group];
-        h.beta1 = y.beta1, h.rest1 = y.rest1, h.beta2 = y.beta2, h.rest2 = y.rest2;
-        h.lr_decay = y.lr_decay, h.eps = y.eps;
-        // 1 - b^t without the cancellation of 1 - pow(b, t)
-        h.step_size = y.lr / -expm1f(steps * y.log_beta1);
-        h.root_scale = rsqrtf(-expm1f(steps * y.log_beta2));
-        adam_part<kF32>(e, {max(int64_t(e.lead), int64_t(tile - tab.first[t]) * kAdamTile),
-                            min(e.end, int64_t(stop - tab.first[t]) * kAdamTile)}, h);
-        tile = stop;
+        const int64_t at = int64_t(tile - tab.first[t]) * kAdamTile;
+        adam_part<kF32>(e, {max(int64_t(e.lead), at), min(e.end, at + kAdamTile)}, h);
     }
     if (call.advance) {
         // the last block to come counts the update: all have read step[0] by then
