@@ -49,12 +49,16 @@ __device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float x)
 }
 
 // ---------------------------------------------------------------- tables --
-// A tensor is numbered from the 16-byte boundary at or below its first
-// element: its elements are the numbers [lead, end) from `base`, whatever its
-// offset, and every 16 bytes in between are one aligned vector.  Tile k holds
+// A tensor is numbered from the line boundary (128 bytes) at or below its
+// first element: its elements are the numbers [lead, end) from `base`,
+// whatever its offset.  The elements before the next boundary and those after
+// the last whole vector go one by one, all others as aligned vectors of which
+// a warp's 32 fill whole lines (from 16-byte boundaries, a warp's load spans
+// five lines for four, and two warps write parts of one).  Tile k holds
 // the numbers [k * tile, (k + 1) * tile); tensor t of a table owns the tiles
 // [first[t], first[t + 1]) of the launch.
 constexpr int kTileBytes = 16384;
+constexpr int kLine = 128;
 
 template <int N>
 struct SpanTable {
@@ -147,7 +151,8 @@ template <int P, int D>
 __device__ __forceinline__ double reduce_part(const void* base, Part part) {
     constexpr int V = 16 / elem_size(D);  // elements of a vector
     constexpr int kUnroll = 4;
-    const int64_t first = (part.lo + V - 1) / V, last = part.hi / V;  // whole vectors
+    constexpr int L = kLine / elem_size(D);
+    const int64_t first = (part.lo + L - 1) / L * (L / V), last = part.hi / V;  // whole vectors
     const uint4* vec = static_cast<const uint4*>(base) + first;
     const int n = int(max(last - first, int64_t(0)));  // a block's part is below 2^31 vectors
     double acc = 0.0;
@@ -203,10 +208,10 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part) {
         const uint32_t one = D == XSG_F32 ? top : max(top & 0xffffu, top >> 16);
         acc = double(D == XSG_F32 ? __uint_as_float(one) : halves(one, D).x);
     }
-    // the elements before the first and after the last whole vector
+    // the elements before the first and after the last of these vectors, each fewer than a line's
     const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
-    const int64_t odd = threadIdx.x < V ? part.lo + threadIdx.x : tail + threadIdx.x - V;
-    if (threadIdx.x < 2 * V && odd < (threadIdx.x < V ? head : part.hi))
+    const int64_t odd = threadIdx.x < L ? part.lo + threadIdx.x : tail + threadIdx.x - L;
+    if (threadIdx.x < 2 * L && odd < (threadIdx.x < L ? head : part.hi))
         acc = join<P>(acc, term<P>(load_as(base, D, odd)));
     return acc;
 }
@@ -329,7 +334,8 @@ template <int D>
 __device__ __forceinline__ void scale_part(void* base, Part part, float c) {
     constexpr int V = 16 / elem_size(D);
     constexpr int kUnroll = 4, kStep = kUnroll * kOptThreads;
-    const int64_t first = (part.lo + V - 1) / V, last = part.hi / V;
+    constexpr int L = kLine / elem_size(D);
+    const int64_t first = (part.lo + L - 1) / L * (L / V), last = part.hi / V;
     uint4* vec = static_cast<uint4*>(base) + first;
     const int n = int(max(last - first, int64_t(0)));  // a block's part is below 2^31 vectors
     int i = n / kStep * kStep + threadIdx.x;
@@ -347,8 +353,8 @@ __device__ __forceinline__ void scale_part(void* base, Part part, float c) {
                 make_uint4(scaled<D>(q[k].x, c), scaled<D>(q[k].y, c), scaled<D>(q[k].z, c), scaled<D>(q[k].w, c));
     }
     const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
-    const int64_t odd = threadIdx.x < V ? part.lo + threadIdx.x : tail + threadIdx.x - V;
-    if (threadIdx.x < 2 * V && odd < (threadIdx.x < V ? head : part.hi))
+    const int64_t odd = threadIdx.x < L ? part.lo + threadIdx.x : tail + threadIdx.x - L;
+    if (threadIdx.x < 2 * L && odd < (threadIdx.x < L ? head : part.hi))
         store_as(base, D, odd, load_as(base, D, odd) * c);
 }
 
@@ -381,6 +387,7 @@ __global__ void __launch_bounds__(kOptThreads, kOptResident)
 
 // ----------------------------------------------------------------- AdamW --
 constexpr int kAdamTile = 4096;  // elements
+constexpr int kAdamLine = 64;     // elements: whole lines for every type
 constexpr int kAdamResident = 4;  // blocks an SM
 constexpr int kAdamGroups = 32;
 
@@ -390,9 +397,10 @@ struct AdamHyper {
 };
 
 // Elements are numbered from `lead` on, as above, in vectors of four; the
-// pointers are those of number 0.  All arrays of a tensor have to have the
-// same lead for that (`vec`); where they do not, lead is 0 and elements go
-// one by one.
+// pointers are those of number 0, which is a multiple of 64 elements for the
+// parameter.  All arrays of a tensor have to be as far past a multiple of
+// four elements for that (`vec`); where they are not, lead is 0 and elements
+// go one by one.
 struct AdamEntry {
     void* param;
     const void* grad;
@@ -492,7 +500,8 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
         for (int64_t i = part.lo + threadIdx.x; i < part.hi; i += kOptThreads) one(i);
         return;
     }
-    const int64_t first = (part.lo + 3) / 4, last = part.hi / 4;
+    constexpr int L = kAdamLine;
+    const int64_t first = (part.lo + L - 1) / L * (L / 4), last = part.hi / 4;
     const int n = int(max(last - first, int64_t(0)));
     const uint32_t skew = rem0 + uint32_t(4 * first - part.lo);  // of vector 0 from the row's start
     for (int at = threadIdx.x; at < n; at += kOptThreads) {
@@ -534,8 +543,8 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
         }
     }
     const int64_t head = min(first * 4, part.hi), tail = max(last * 4, head);
-    const int64_t odd = threadIdx.x < 4 ? part.lo + threadIdx.x : tail + threadIdx.x - 4;
-    if (threadIdx.x < 8 && odd < (threadIdx.x < 4 ? head : part.hi)) one(odd);
+    const int64_t odd = threadIdx.x < L ? part.lo + threadIdx.x : tail + threadIdx.x - L;
+    if (threadIdx.x < 2 * L && odd < (threadIdx.x < L ? head : part.hi)) one(odd);
 }
 
 template <int N, bool kF32>
@@ -614,18 +623,13 @@ int check_spans(const xsg_span* spans, int64_t n, const char* what) {
     return XSG_OK;
 }
 
-// The element that the arrays of an update have in common as their first past
-// a vector's boundary, or -1 if they have none.
+// How far the parameter is past a multiple of 64 elements, or -1 if another
+// array of the update is not as far past a multiple of four.
 int common_lead(const xsg_adamw_span& s) {
-    int lead = -1;
-    const auto same = [&](const void* p, int size) {
-        const int l = int(reinterpret_cast<uintptr_t>(p) / size % 4);
-        const bool ok = lead < 0 || l == lead;
-        lead = l;
-        return ok;
-    };
-    const bool all = same(s.param, elem_size(s.param_dtype)) && same(s.grad, elem_size(s.grad_dtype)) &&
-                     same(s.exp_avg, 4) && same(s.exp_avg_sq, 4) && (!s.master || same(s.master, 4));
+    const auto past = [](const void* p, int size, int of) { return int(reinterpret_cast<uintptr_t>(p) / size % of); };
+    const int lead = past(s.param, elem_size(s.param_dtype), kAdamLine);
+    const bool all = past(s.grad, elem_size(s.grad_dtype), 4) == lead % 4 && past(s.exp_avg, 4, 4) == lead % 4 &&
+                     past(s.exp_avg_sq, 4, 4) == lead % 4 && (!s.master || past(s.master, 4, 4) == lead % 4);
     return all ? lead : -1;
 }
 
@@ -642,8 +646,8 @@ std::vector<SpanLaunch> plan_spans(const xsg_span* spans, int64_t n) {
             const xsg_span& s = spans[L.first_span + t];
             const int64_t per = kTileBytes / elem_size(s.dtype);
             const auto at = reinterpret_cast<uintptr_t>(s.data);
-            const int64_t lead = int64_t(at % 16) / elem_size(s.dtype);
-            L.tab.base[t] = reinterpret_cast<void*>(at - at % 16);
+            const int64_t lead = int64_t(at % kLine) / elem_size(s.dtype);
+            L.tab.base[t] = reinterpret_cast<void*>(at - at % kLine);
             L.tab.lead[t] = uint8_t(lead);
             L.tab.end[t] = lead + s.n;
             L.tab.dtype[t] = uint8_t(s.dtype);
