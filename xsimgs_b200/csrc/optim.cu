@@ -13,6 +13,7 @@
 // contiguous run of the tiles of all tensors, so that tensors of any size
 // share the work evenly and the order of every sum depends on the tensors'
 // sizes alone: no atomics, the same bits on every run.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -20,9 +21,12 @@
 #include <cmath>
 #include <cstring>
 #include <exception>
+#include <type_traits>
 #include <vector>
 
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace xsg {
 namespace {
@@ -80,11 +84,12 @@ __device__ __forceinline__ Part part_of(const Table& tab, int t, int32_t tile, i
     return {max(int64_t(tab.lead[t]), (tile - tab.first[t]) * per), min(tab.end[t], (stop - tab.first[t]) * per)};
 }
 
-// The run of tiles of block b out of `blocks`, and back.
-__host__ __device__ __forceinline__ int32_t run_start(int32_t tiles, int32_t blocks, int32_t b) {
+// The contiguous run of tiles of block b out of `blocks`, and the block whose
+// run holds a tile.
+__device__ __forceinline__ int32_t run_start(int32_t tiles, int32_t blocks, int32_t b) {
     return int32_t(int64_t(tiles) * b / blocks);
 }
-__host__ __device__ __forceinline__ int32_t block_of(int32_t tiles, int32_t blocks, int32_t tile) {
+__device__ __forceinline__ int32_t run_of(int32_t tiles, int32_t blocks, int32_t tile) {
     return int32_t(((int64_t(tile) + 1) * blocks - 1) / tiles);
 }
 
@@ -147,7 +152,7 @@ __device__ __forceinline__ void add16(double& acc, const float (&x)[16]) {
 }
 
 // Sum (or maximum) over the numbers [lo, hi) of a tensor, by the block.
-template <int P, int D>
+template <int P, int D, int T>
 __device__ __forceinline__ double reduce_part(const void* base, Part part) {
     constexpr int V = 16 / elem_size(D);  // elements of a vector
     constexpr int kUnroll = 4;
@@ -191,17 +196,17 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part) {
         }
     };
     int i = threadIdx.x;
-    for (; i + (kUnroll - 1) * kOptThreads < n; i += kUnroll * kOptThreads) {
+    for (; i + (kUnroll - 1) * T < n; i += kUnroll * T) {
         uint4 q[kUnroll];
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) q[k] = __ldg(vec + i + k * kOptThreads);
+        for (int k = 0; k < kUnroll; ++k) q[k] = vec[i + k * T];
         take(q);
     }
     if (i < n) {
         uint4 q[kUnroll];
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k)
-            q[k] = i + k * kOptThreads < n ? __ldg(vec + i + k * kOptThreads) : make_uint4(0, 0, 0, 0);
+            q[k] = i + k * T < n ? vec[i + k * T] : make_uint4(0, 0, 0, 0);
         take(q);
     }
     if constexpr (P == kNormInf) {
@@ -216,11 +221,11 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part) {
     return acc;
 }
 
-template <int P>
+template <int P, int T>
 __device__ __forceinline__ double reduce_part(const void* base, int dtype, Part part) {
-    if (dtype == XSG_F32) return reduce_part<P, XSG_F32>(base, part);
-    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16>(base, part);
-    return reduce_part<P, XSG_F16>(base, part);
+    if (dtype == XSG_F32) return reduce_part<P, XSG_F32, T>(base, part);
+    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16, T>(base, part);
+    return reduce_part<P, XSG_F16, T>(base, part);
 }
 
 // Over the block, in a fixed order; every thread gets the result.  `smem`
@@ -249,68 +254,81 @@ __device__ __forceinline__ float clip_coefficient(float norm, float max_norm) {
     return c >= 1.f ? 1.f : c;  // a NaN stays
 }
 
-// Partial sums of a launch: sums[b] for the whole run of block b and, where
-// each tensor's norm is asked for, slots[b + t] for its part of tensor t
-// (b + t grows along the runs, so that no two parts share a slot).
+// Partial sums of a launch: sums[b] of all tiles of block b, which takes them
+// in turn.
 template <int P, int N>
 __global__ void __launch_bounds__(kOptThreads, kOptResident)
-    norm_partial_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums,
-                        double* __restrict__ slots) {
+    norm_partial_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums) {
     __shared__ double smem[33];
+    pdl_trigger();
     const int32_t tiles = tab.first[tab.count];
+    double acc = 0.0;
+    int t = -1;
+    for (int32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        if (t < 0) t = owner_of(tab, tile);
+        while (tile >= tab.first[t + 1]) ++t;
+        acc = join<P>(acc, reduce_part<P, kOptThreads>(tab.base[t], tab.dtype[t], part_of(tab, t, tile, tile + 1)));
+    }
+    acc = block_reduce<P>(acc, smem);
+    if (threadIdx.x == 0) sums[blockIdx.x] = acc;
+}
+
+// The same where each tensor's norm is asked for.  A block takes a contiguous
+// run of tiles, and slots[b + t] is its part of tensor t: b + t grows along
+// the runs, so that no two parts share a slot, and blocks + tensors of them
+// are enough.
+template <int P, int N>
+__global__ void __launch_bounds__(kOptThreads, kOptResident)
+    norm_partial_each_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums,
+                             double* __restrict__ slots) {
+    __shared__ double smem[33];
+    pdl_trigger();
+    const int32_t tiles = tab.first[tab.count], end = run_start(tiles, gridDim.x, blockIdx.x + 1);
     int32_t tile = run_start(tiles, gridDim.x, blockIdx.x);
-    const int32_t end = run_start(tiles, gridDim.x, blockIdx.x + 1);
     double whole = 0.0;
     for (int t = owner_of(tab, tile); tile < end; ++t) {
         const int32_t stop = min(end, tab.first[t + 1]);
         if (stop <= tile) continue;
-        double acc = reduce_part<P>(tab.base[t], tab.dtype[t], part_of(tab, t, tile, stop));
-        if (slots) {
-            acc = block_reduce<P>(acc, smem);
-            if (threadIdx.x == 0) slots[blockIdx.x + t] = acc;
-            whole = join<P>(whole, acc);
-        } else {
-            whole = join<P>(whole, acc);
-        }
+        const double acc = block_reduce<P>(
+            reduce_part<P, kOptThreads>(tab.base[t], tab.dtype[t], part_of(tab, t, tile, stop)), smem);
+        if (threadIdx.x == 0) slots[blockIdx.x + t] = acc;
+        whole = join<P>(whole, acc);
         tile = stop;
     }
-    if (!slots) whole = block_reduce<P>(whole, smem);
     if (threadIdx.x == 0) sums[blockIdx.x] = whole;
 }
 
-// All partial sums of a call, by every block for itself.
+// All partial sums of a call, by every block for itself.  (The first pass may
+// still run when a kernel that reads them starts: plain loads, after pdl_wait.)
 template <int P>
 __device__ __forceinline__ float total_norm(const double* sums, int n, double* smem) {
     double v = 0.0;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) v = join<P>(v, sums[i]);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) v = join<P>(v, __ldcg(sums + i));
     return root<P>(block_reduce<P>(v, smem));
 }
 
-// Block 0: the norm of all tensors (if `norm`).  The others: a warp for each
-// tensor of the table.
+// Block 0: the norm of all tensors (if `norm`).  The others: a tensor each.
 template <int P, int N>
 __global__ void __launch_bounds__(kOptThreads)
-    norm_finish_kernel(const __grid_constant__ SpanTable<N> tab, int blocks, const double* __restrict__ sums,
-                       int n_sums, const double* __restrict__ slots, float* __restrict__ norm,
+    norm_finish_kernel(const __grid_constant__ SpanTable<N> tab, int blocks, const double* sums,
+                       int n_sums, const double* slots, float* __restrict__ norm,
                        float* __restrict__ norms) {
     __shared__ double smem[33];
+    pdl_wait();
     if (blockIdx.x == 0) {
         if (!norm) return;
         const float v = total_norm<P>(sums, n_sums, smem);
         if (threadIdx.x == 0) *norm = v;
         return;
     }
-    const int t = (blockIdx.x - 1) * (kOptThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (t >= tab.count) return;
-    double v = 0.0;
-    const int32_t tiles = tab.first[tab.count];
-    if (tab.first[t + 1] > tab.first[t]) {
-        const int b0 = block_of(tiles, blocks, tab.first[t]), b1 = block_of(tiles, blocks, tab.first[t + 1] - 1);
-        for (int b = b0 + lane; b <= b1; b += 32) v = join<P>(v, slots[b + t]);
+    const int t = blockIdx.x - 1;
+    const int32_t tiles = tab.first[tab.count], begin = tab.first[t], end = tab.first[t + 1];
+    float v = 0.f;
+    if (end > begin) {
+        const int b0 = run_of(tiles, blocks, begin), b1 = run_of(tiles, blocks, end - 1);
+        v = total_norm<P>(slots + b0 + t, b1 - b0 + 1, smem);
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = join<P>(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if (lane == 0) norms[t] = root<P>(v);
+    if (threadIdx.x == 0) norms[t] = v;
 }
 
 // g <- c g over the numbers [lo, hi) of a tensor, by the block, from the end
@@ -330,26 +348,26 @@ __device__ __forceinline__ uint32_t scaled(uint32_t w, float c) {
     return r;
 }
 
-template <int D>
+template <int D, int T>
 __device__ __forceinline__ void scale_part(void* base, Part part, float c) {
     constexpr int V = 16 / elem_size(D);
-    constexpr int kUnroll = 4, kStep = kUnroll * kOptThreads;
+    constexpr int kUnroll = 4, kStep = kUnroll * T;
     constexpr int L = kLine / elem_size(D);
     const int64_t first = (part.lo + L - 1) / L * (L / V), last = part.hi / V;
     uint4* vec = static_cast<uint4*>(base) + first;
     const int n = int(max(last - first, int64_t(0)));  // a block's part is below 2^31 vectors
     int i = n / kStep * kStep + threadIdx.x;
-    for (int j = i; j < n; j += kOptThreads) {
+    for (int j = i; j < n; j += T) {
         const uint4 q = vec[j];
         vec[j] = make_uint4(scaled<D>(q.x, c), scaled<D>(q.y, c), scaled<D>(q.z, c), scaled<D>(q.w, c));
     }
     for (i -= kStep; i >= 0; i -= kStep) {
         uint4 q[kUnroll];
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) q[k] = vec[i + k * kOptThreads];
+        for (int k = 0; k < kUnroll; ++k) q[k] = vec[i + k * T];
 #pragma unroll
         for (int k = 0; k < kUnroll; ++k)
-            vec[i + k * kOptThreads] =
+            vec[i + k * T] =
                 make_uint4(scaled<D>(q[k].x, c), scaled<D>(q[k].y, c), scaled<D>(q[k].z, c), scaled<D>(q[k].w, c));
     }
     const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
@@ -358,30 +376,123 @@ __device__ __forceinline__ void scale_part(void* base, Part part, float c) {
         store_as(base, D, odd, load_as(base, D, odd) * c);
 }
 
-// The second pass of clipping.  c = 1 leaves the data alone.  Every block
-// takes the run that it had in the first pass, backwards, so that what the
-// first pass read last, and the L2 still holds, comes first.
+template <int T, typename Table>
+__device__ __forceinline__ void scale_part(const Table& tab, int t, Part part, float c) {
+    const int dtype = tab.dtype[t];
+    if (dtype == XSG_F32) scale_part<XSG_F32, T>(tab.base[t], part, c);
+    else if (dtype == XSG_BF16) scale_part<XSG_BF16, T>(tab.base[t], part, c);
+    else scale_part<XSG_F16, T>(tab.base[t], part, c);
+}
+
+// The second pass of clipping.  c = 1 leaves the data alone.  The tiles are
+// taken from the last to the first, so that what the first pass read last,
+// and the L2 still holds, comes first.
 template <int P, int N>
 __global__ void __launch_bounds__(kOptThreads, kOptResident)
-    clip_scale_kernel(const __grid_constant__ SpanTable<N> tab, const double* __restrict__ sums, int n_sums,
+    clip_scale_kernel(const __grid_constant__ SpanTable<N> tab, const double* sums, int n_sums,
                       float max_norm, float* __restrict__ norm) {
     __shared__ double smem[33];
+    pdl_wait();
     const float total = total_norm<P>(sums, n_sums, smem);
     if (blockIdx.x == 0 && threadIdx.x == 0 && norm) *norm = total;
     const float c = clip_coefficient(total, max_norm);
     if (c == 1.f) return;
-    const int32_t tiles = tab.first[tab.count];
-    const int32_t begin = run_start(tiles, gridDim.x, blockIdx.x);
-    int32_t stop = run_start(tiles, gridDim.x, blockIdx.x + 1);
-    for (int t = owner_of(tab, stop - 1); stop > begin; --t) {
-        const int32_t tile = max(begin, tab.first[t]);
-        if (tile >= stop) continue;
-        const Part part = part_of(tab, t, tile, stop);
-        const int dtype = tab.dtype[t];
-        if (dtype == XSG_F32) scale_part<XSG_F32>(tab.base[t], part, c);
-        else if (dtype == XSG_BF16) scale_part<XSG_BF16>(tab.base[t], part, c);
-        else scale_part<XSG_F16>(tab.base[t], part, c);
-        stop = tile;
+    int t = -1;
+    for (int32_t tile = tab.first[tab.count] - 1 - int32_t(blockIdx.x); tile >= 0; tile -= gridDim.x) {
+        if (t < 0) t = owner_of(tab, tile);
+        while (tile < tab.first[t]) --t;
+        scale_part<kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), c);
+    }
+}
+
+// --------------------------------------------------------- small tensors --
+// What eight SMs read in a few microseconds goes in one launch: a cluster of
+// blocks, each with a run of the tiles; the blocks' sums meet in shared
+// memory over the cluster, and each block scales what it has just read.
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallBlocks = 8;
+constexpr int kSmallSpans = 32;
+
+// A block's sums, where the others of the cluster read them.
+struct ClusterSums {
+    double whole;
+    double each[kSmallSpans];
+    double smem[33];
+};
+
+// Over the cluster, in the order of the ranks; every thread gets it.
+template <int P>
+__device__ __forceinline__ double cluster_join(cg::cluster_group& cluster, double* mine) {
+    double v = 0.0;
+    for (unsigned r = 0; r < cluster.num_blocks(); ++r) v = join<P>(v, *cluster.map_shared_rank(mine, r));
+    return v;
+}
+
+// The sum over this block's run of tiles.
+template <int P, bool kEach>
+__device__ __forceinline__ void run_sums(const SpanTable<kSmallSpans>& tab, int32_t rank, int32_t ranks,
+                                         ClusterSums& s) {
+    const int32_t tiles = tab.first[tab.count], end = run_start(tiles, ranks, rank + 1);
+    int32_t tile = run_start(tiles, ranks, rank);
+    if (kEach) {
+        if (threadIdx.x < kSmallSpans) s.each[threadIdx.x] = 0.0;
+        __syncthreads();
+    }
+    double acc = 0.0, whole = 0.0;
+    for (int t = owner_of(tab, tile); tile < end; ++t) {
+        const int32_t stop = min(end, tab.first[t + 1]);
+        if (stop <= tile) continue;
+        acc = join<P>(acc, reduce_part<P, kSmallThreads>(tab.base[t], tab.dtype[t], part_of(tab, t, tile, stop)));
+        if (kEach) {
+            acc = block_reduce<P>(acc, s.smem);
+            if (threadIdx.x == 0) s.each[t] = acc;
+            whole = join<P>(whole, acc);
+            acc = 0.0;
+        }
+        tile = stop;
+    }
+    if (!kEach) whole = block_reduce<P>(acc, s.smem);
+    if (threadIdx.x == 0) s.whole = whole;
+}
+
+template <int P>
+__global__ void __launch_bounds__(kSmallThreads)
+    norm_small_kernel(const __grid_constant__ SpanTable<kSmallSpans> tab, float* __restrict__ norm,
+                      float* __restrict__ norms) {
+    __shared__ ClusterSums sums;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank());
+    if (norms) run_sums<P, true>(tab, rank, int(cluster.num_blocks()), sums);
+    else run_sums<P, false>(tab, rank, int(cluster.num_blocks()), sums);
+    cluster.sync();
+    if (rank == 0) {
+        if (threadIdx.x == 0) *norm = root<P>(cluster_join<P>(cluster, &sums.whole));
+        if (norms && int(threadIdx.x) >= 32 && int(threadIdx.x) < 32 + tab.count)
+            norms[threadIdx.x - 32] = root<P>(cluster_join<P>(cluster, &sums.each[threadIdx.x - 32]));
+    }
+    cluster.sync();  // the others' sums stay until they are read
+}
+
+template <int P>
+__global__ void __launch_bounds__(kSmallThreads)
+    clip_small_kernel(const __grid_constant__ SpanTable<kSmallSpans> tab, float max_norm, float* __restrict__ norm) {
+    __shared__ ClusterSums sums;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank()), ranks = int(cluster.num_blocks());
+    run_sums<P, false>(tab, rank, ranks, sums);
+    cluster.sync();
+    const float total = root<P>(cluster_join<P>(cluster, &sums.whole));
+    cluster.sync();
+    if (rank == 0 && threadIdx.x == 0) *norm = total;
+    const float c = clip_coefficient(total, max_norm);
+    if (c == 1.f) return;
+    const int32_t tiles = tab.first[tab.count], end = run_start(tiles, ranks, rank + 1);
+    int32_t tile = run_start(tiles, ranks, rank);
+    for (int t = owner_of(tab, tile); tile < end; ++t) {
+        const int32_t stop = min(end, tab.first[t + 1]);
+        if (stop <= tile) continue;
+        scale_part<kSmallThreads>(tab, t, part_of(tab, t, tile, stop), c);
+        tile = stop;
     }
 }
 
@@ -476,7 +587,7 @@ __device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const floa
 // The update over the numbers [lo, hi) of a tensor, by the block.  kF32: all
 // arrays are in 32 bits and there is no master, so no branch on the types
 // stands between the loads.
-template <bool kF32>
+template <bool kF32, int T>
 __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const AdamScale& h) {
     const int pd = kF32 ? XSG_F32 : e.param_dtype, gd = kF32 ? XSG_F32 : e.grad_dtype;
     float* master = kF32 ? nullptr : e.master;
@@ -497,14 +608,14 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
         store_as(e.param, pd, i, w);
     };
     if (!e.vec) {
-        for (int64_t i = part.lo + threadIdx.x; i < part.hi; i += kOptThreads) one(i);
+        for (int64_t i = part.lo + threadIdx.x; i < part.hi; i += T) one(i);
         return;
     }
     constexpr int L = kAdamLine;
     const int64_t first = (part.lo + L - 1) / L * (L / 4), last = part.hi / 4;
     const int n = int(max(last - first, int64_t(0)));
     const uint32_t skew = rem0 + uint32_t(4 * first - part.lo);  // of vector 0 from the row's start
-    for (int at = threadIdx.x; at < n; at += kOptThreads) {
+    for (int at = threadIdx.x; at < n; at += T) {
         uint32_t keep = 15u;
         if (e.rows) {
             const uint32_t x = skew + 4u * uint32_t(at), r = x / rs, rem = x - r * rs;
@@ -547,26 +658,15 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
     if (threadIdx.x < 2 * L && odd < (threadIdx.x < L ? head : part.hi)) one(odd);
 }
 
-template <int N, bool kF32>
-__global__ void __launch_bounds__(kOptThreads, kAdamResident)
-    adamw_kernel(const __grid_constant__ AdamTable<N> tab, const __grid_constant__ AdamCall call) {
-    __shared__ double smem[33];
-    AdamScale h;
-    h.c = 1.f;
-    if (call.sums) {
-        const float total = total_norm<2>(call.sums, call.n_sums, smem);
-        if (blockIdx.x == 0 && threadIdx.x == 0 && call.norm) *call.norm = total;
-        if (call.skip_nonfinite && !isfinite(total)) return;  // every block alike: nothing changes
-        if (call.clip) h.c = clip_coefficient(total, call.max_norm);
-    }
-    const float steps = float(call.step[0] + 1);
-    // tiles in turn: a part of a masked tensor may have little to do
-    const int32_t tiles = tab.first[tab.count];
+// The tiles of block b of `blocks`, in turn (a part of a masked tensor may
+// have little to do) and from the last to the first, as in clipping.
+template <bool kF32, int T, typename Table>
+__device__ __forceinline__ void adam_tiles(const Table& tab, int32_t b, int32_t blocks, float steps, AdamScale& h) {
     int t = -1;
-    for (int32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        if (t < 0 || tile >= tab.first[t + 1]) {
+    for (int32_t tile = tab.first[tab.count] - 1 - b; tile >= 0; tile -= blocks) {
+        if (t < 0 || tile < tab.first[t]) {
             if (t < 0) t = owner_of(tab, tile);
-            while (tile >= tab.first[t + 1]) ++t;
+            while (tile < tab.first[t]) --t;
             const AdamHyper& y = tab.hyper[tab.entry[t].group];
             h.beta1 = y.beta1, h.rest1 = y.rest1, h.beta2 = y.beta2, h.rest2 = y.rest2;
             h.lr_decay = y.lr_decay, h.eps = y.eps;
@@ -576,36 +676,100 @@ __global__ void __launch_bounds__(kOptThreads, kAdamResident)
         }
         const AdamEntry& e = tab.entry[t];
         const int64_t at = int64_t(tile - tab.first[t]) * kAdamTile;
-        adam_part<kF32>(e, {max(int64_t(e.lead), at), min(e.end, at + kAdamTile)}, h);
+        adam_part<kF32, T>(e, {max(int64_t(e.lead), at), min(e.end, at + kAdamTile)}, h);
     }
-    if (call.advance) {
-        // the last block to come counts the update: all have read step[0] by then
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            auto* word = reinterpret_cast<unsigned long long*>(call.step);
-            if (atomicAdd(word + 1, 1ull) == gridDim.x - 1) {
-                word[0] += 1;
-                word[1] = 0;
-            }
+}
+
+// The last of the blocks to come counts the update: all have read step[0] by then.
+__device__ __forceinline__ void count_update(long long* step) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        auto* word = reinterpret_cast<unsigned long long*>(step);
+        if (atomicAdd(word + 1, 1ull) == gridDim.x - 1) {
+            word[0] += 1;
+            word[1] = 0;
         }
     }
+}
+
+template <int N, bool kF32>
+__global__ void __launch_bounds__(kOptThreads, kAdamResident)
+    adamw_kernel(const __grid_constant__ AdamTable<N> tab, const __grid_constant__ AdamCall call) {
+    __shared__ double smem[33];
+    AdamScale h;
+    h.c = 1.f;
+    if (call.sums) {
+        pdl_wait();
+        const float total = total_norm<2>(call.sums, call.n_sums, smem);
+        if (blockIdx.x == 0 && threadIdx.x == 0 && call.norm) *call.norm = total;
+        if (call.skip_nonfinite && !isfinite(total)) return;  // every block alike: nothing changes
+        if (call.clip) h.c = clip_coefficient(total, call.max_norm);
+    }
+    adam_tiles<kF32, kOptThreads>(tab, blockIdx.x, gridDim.x, float(call.step[0] + 1), h);
+    if (call.advance) count_update(call.step);
+}
+
+// Norm and update of small tensors in one launch (see norm_small_kernel).
+template <bool kF32>
+__global__ void __launch_bounds__(kSmallThreads)
+    adamw_small_kernel(const __grid_constant__ SpanTable<kSmallSpans> grads,
+                       const __grid_constant__ AdamTable<kSmallSpans> tab, const __grid_constant__ AdamCall call) {
+    __shared__ ClusterSums sums;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = int(cluster.block_rank()), ranks = int(cluster.num_blocks());
+    run_sums<2, false>(grads, rank, ranks, sums);
+    cluster.sync();
+    const float total = root<2>(cluster_join<2>(cluster, &sums.whole));
+    const float steps = float(call.step[0] + 1);
+    cluster.sync();
+    if (rank == 0 && threadIdx.x == 0 && call.norm) *call.norm = total;
+    if (call.skip_nonfinite && !isfinite(total)) return;
+    AdamScale h;
+    h.c = call.clip ? clip_coefficient(total, call.max_norm) : 1.f;
+    adam_tiles<kF32, kSmallThreads>(tab, rank, ranks, steps, h);
+    if (rank == 0 && threadIdx.x == 0) call.step[0] += 1;  // all blocks have read it
 }
 
 // ------------------------------------------------------------------ host --
 constexpr int kSpans = 1024;
 constexpr int kAdamSpans = 400;
-static_assert(sizeof(SpanTable<kSpans>) <= 32000 && sizeof(AdamTable<kAdamSpans>) <= 32000,
+static_assert(sizeof(SpanTable<kSpans>) <= 32000 && sizeof(AdamTable<kAdamSpans>) + sizeof(AdamCall) <= 32000,
               "kernel parameters hold 32764 bytes");
+// One launch of a cluster against two of the whole GPU.
+constexpr int64_t kSmallNormBytes = 1 << 20;
+constexpr int64_t kSmallAdamElems = 1 << 16;
 
-struct SpanLaunch {
-    SpanTable<kSpans> tab;
-    int blocks = 0;
-    int64_t first_span = 0, sums_at = 0, slots_at = 0;
+template <typename T>
+struct Same {
+    using type = T;
 };
 
-bool known_dtype(int d) { return d == XSG_F32 || d == XSG_BF16 || d == XSG_F16; }
+// A launch by reference: the tables are copied once, by the driver.
+template <typename... P>
+void launch_table(void (*kernel)(P...), unsigned grid, unsigned block, unsigned cluster, bool pdl, cudaStream_t st,
+                  const typename Same<P>::type&... args) {
+    count_launch();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    cfg.attrs = attr;
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim = {cluster, 1, 1};
+        ++cfg.numAttrs;
+    }
+    if (pdl) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+    }
+    void* pointers[] = {const_cast<void*>(static_cast<const void*>(&args))...};
+    (void)cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kernel), pointers);  // errors surface in check_launch
+}
 
-int64_t span_launches(int64_t n_spans) { return (n_spans + kSpans - 1) / kSpans; }
+bool known_dtype(int d) { return d == XSG_F32 || d == XSG_BF16 || d == XSG_F16; }
 
 constexpr int64_t kMaxElems = int64_t(1) << 40;  // keeps tile numbers inside 31 bits
 
@@ -623,152 +787,176 @@ int check_spans(const xsg_span* spans, int64_t n, const char* what) {
     return XSG_OK;
 }
 
-// How far the parameter is past a multiple of 64 elements, or -1 if another
-// array of the update is not as far past a multiple of four.
-int common_lead(const xsg_adamw_span& s) {
-    const auto past = [](const void* p, int size, int of) { return int(reinterpret_cast<uintptr_t>(p) / size % of); };
-    const int lead = past(s.param, elem_size(s.param_dtype), kAdamLine);
-    const bool all = past(s.grad, elem_size(s.grad_dtype), 4) == lead % 4 && past(s.exp_avg, 4, 4) == lead % 4 &&
-                     past(s.exp_avg_sq, 4, 4) == lead % 4 && (!s.master || past(s.master, 4, 4) == lead % 4);
-    return all ? lead : -1;
-}
+// The tensors of one launch.
+template <int N>
+struct SpanLaunch {
+    SpanTable<N> tab;
+    int blocks = 0;
+    int64_t first_span = 0, sums_at = 0, slots_at = 0, bytes = 0;
 
-// Cuts the spans into launches of at most kSpans tensors.
-std::vector<SpanLaunch> plan_spans(const xsg_span* spans, int64_t n) {
-    std::vector<SpanLaunch> out(span_launches(n));
+    void add(const void* data, int64_t n, int dtype) {
+        const int t = tab.count;
+        const int64_t per = kTileBytes / elem_size(dtype);
+        const auto at = reinterpret_cast<uintptr_t>(data);
+        const int64_t lead = int64_t(at % kLine) / elem_size(dtype);
+        tab.base[t] = reinterpret_cast<void*>(at - at % kLine);
+        tab.lead[t] = uint8_t(lead);
+        tab.end[t] = lead + n;
+        tab.dtype[t] = uint8_t(dtype);
+        bytes += n * elem_size(dtype);
+        tab.first[t + 1] = int32_t(tab.first[t] + (n ? (lead + n + per - 1) / per : 0));
+        tab.count = t + 1;
+    }
+    // Blocks and slots, when all tensors are in.
+    void close(int64_t& sums, int64_t& slots) {
+        const int32_t tiles = tab.first[tab.count];
+        blocks = std::max(1, std::min(tiles, kOptBlocks));
+        sums_at = sums;
+        sums += blocks;
+        slots_at = slots;
+        slots += blocks + tab.count;
+    }
+    SpanLaunch() {
+        tab.count = 0;
+        tab.first[0] = 0;
+    }
+};
+
+size_t sums_count(int64_t n_spans) { return size_t((n_spans + kSpans - 1) / kSpans) * kOptBlocks; }
+size_t slots_count(int64_t n_spans) { return sums_count(n_spans) + size_t(n_spans); }
+
+// All launches over `n` tensors, tensor i from get(i): one of a small table
+// where that holds them, else as many of the large table as it takes.
+template <int N>
+struct SpanPlan {
+    std::vector<SpanLaunch<N>> launches;
     int64_t sums = 0, slots = 0;
-    for (size_t l = 0; l < out.size(); ++l) {
-        SpanLaunch& L = out[l];
-        L.first_span = int64_t(l) * kSpans;
-        L.tab.count = int32_t(std::min<int64_t>(kSpans, n - L.first_span));
-        int64_t tiles = 0;
-        for (int t = 0; t < L.tab.count; ++t) {
-            const xsg_span& s = spans[L.first_span + t];
-            const int64_t per = kTileBytes / elem_size(s.dtype);
-            const auto at = reinterpret_cast<uintptr_t>(s.data);
-            const int64_t lead = int64_t(at % kLine) / elem_size(s.dtype);
-            L.tab.base[t] = reinterpret_cast<void*>(at - at % kLine);
-            L.tab.lead[t] = uint8_t(lead);
-            L.tab.end[t] = lead + s.n;
-            L.tab.dtype[t] = uint8_t(s.dtype);
-            L.tab.first[t] = int32_t(tiles);
-            tiles += s.n ? (lead + s.n + per - 1) / per : 0;
+
+    template <typename Get>
+    SpanPlan(int64_t n, Get&& get) : launches((n + N - 1) / N) {
+        for (int64_t i = 0; i < n; ++i) {
+            SpanLaunch<N>& L = launches[i / N];
+            if (L.tab.count == 0) L.first_span = i;
+            get(i, L);
         }
-        L.tab.first[L.tab.count] = int32_t(tiles);
-        L.blocks = int(std::max<int64_t>(1, std::min<int64_t>(tiles, kOptBlocks)));
-        L.sums_at = sums;
-        L.slots_at = slots;
-        sums += L.blocks;
-        slots += L.blocks + L.tab.count;
+        for (auto& L : launches) L.close(sums, slots);
     }
-    return out;
-}
 
-size_t sums_bytes(int64_t n_spans) { return Arena::round(span_launches(n_spans) * kOptBlocks * sizeof(double)); }
-size_t slots_bytes(int64_t n_spans) {
-    return Arena::round((span_launches(n_spans) * kOptBlocks + n_spans) * sizeof(double));
-}
+    bool small(int64_t limit) const { return N == kSmallSpans && launches[0].bytes <= limit; }
 
-template <int P>
-void launch_partials(const std::vector<SpanLaunch>& plan, double* sums, double* slots, cudaStream_t st) {
-    for (const SpanLaunch& L : plan)
-        launch(norm_partial_kernel<P, kSpans>, L.blocks, kOptThreads, 0, st, L.tab, sums + L.sums_at,
-               slots ? slots + L.slots_at : nullptr);
-}
-
-int total_sums(const std::vector<SpanLaunch>& plan) { return int(plan.back().sums_at) + plan.back().blocks; }
-
-template <int P>
-void norm_all(const std::vector<SpanLaunch>& plan, double* sums, double* slots, float* norm, float* norms,
-              cudaStream_t st) {
-    launch_partials<P>(plan, sums, slots, st);
-    for (size_t l = 0; l < plan.size(); ++l) {
-        const SpanLaunch& L = plan[l];
-        const bool last = l + 1 == plan.size();
-        if (!slots && !last) continue;
-        const unsigned grid = 1 + (slots ? blocks_for(L.tab.count, kOptThreads / 32) : 0);
-        launch(norm_finish_kernel<P, kSpans>, grid, kOptThreads, 0, st, L.tab, L.blocks,
-               static_cast<const double*>(sums), total_sums(plan),
-               static_cast<const double*>(slots ? slots + L.slots_at : nullptr), last ? norm : nullptr,
-               norms ? norms + L.first_span : nullptr);
+    unsigned cluster() const {
+        unsigned c = 1;
+        while (c < kSmallBlocks && int32_t(c) < launches[0].blocks) c *= 2;
+        return c;
     }
-}
 
-template <int P>
-void clip_all(const std::vector<SpanLaunch>& plan, double* sums, float max_norm, float* norm, cudaStream_t st) {
-    launch_partials<P>(plan, sums, nullptr, st);
-    for (size_t l = plan.size(); l-- > 0;)
-        launch(clip_scale_kernel<P, kSpans>, plan[l].blocks, kOptThreads, 0, st, plan[l].tab,
-               static_cast<const double*>(sums), total_sums(plan), max_norm, l == 0 ? norm : nullptr);
-}
-
-// No C++ exception leaves a C entry.
-template <typename F>
-int guarded(const char* what, F&& body) {
-    try {
-        return body();
-    } catch (const std::exception& e) {
-        return set_error(XSG_ERR_INVALID_ARGUMENT, std::string(what) + ": " + e.what());
+    template <int P>
+    void partials(double* sums_at, double* slots_at, cudaStream_t st) const {
+        for (const auto& L : launches) {
+            if (slots_at)
+                launch_table(norm_partial_each_kernel<P, N>, L.blocks, kOptThreads, 1, false, st, L.tab,
+                             sums_at + L.sums_at, slots_at + L.slots_at);
+            else
+                launch_table(norm_partial_kernel<P, N>, L.blocks, kOptThreads, 1, false, st, L.tab,
+                             sums_at + L.sums_at);
+        }
     }
-}
+};
 
-}  // namespace
-}  // namespace xsg
-
-using namespace xsg;
-
-extern "C" size_t xsg_grad_norm_workspace_size(int64_t n_spans) {
-    if (n_spans <= 0) return 0;
-    return sums_bytes(n_spans) + slots_bytes(n_spans);
-}
-
-static int grad_norm(const xsg_span* spans_host, int64_t n_spans, int norm_type, float* norm, float* norms,
-                             void* workspace, size_t workspace_bytes, xsg_stream_t stream) {
-    if (int rc = check_spans(spans_host, n_spans, "grad_norm")) return rc;
-    XSG_REQUIRE(norm, "grad_norm: null output");
-    Arena arena(workspace, workspace ? workspace_bytes : 0);
-    double* sums = arena.take<double>(span_launches(n_spans) * kOptBlocks);
-    double* slots = norms ? arena.take<double>(span_launches(n_spans) * kOptBlocks + n_spans) : nullptr;
+template <int P, int N>
+int norm_all(const SpanPlan<N>& plan, float* norm, float* norms, Arena arena, int64_t n, cudaStream_t st) {
+    if constexpr (N == kSmallSpans) {
+        if (plan.small(kSmallNormBytes)) {
+            launch_table(norm_small_kernel<P>, plan.cluster(), kSmallThreads, plan.cluster(), false, st,
+                         plan.launches[0].tab, norm, norms);
+            return XSG_OK;
+        }
+    }
+    double* sums = arena.take<double>(sums_count(n));
+    double* slots = norms ? arena.take<double>(slots_count(n)) : nullptr;
     if (!sums || (norms && !slots)) return set_error(XSG_ERR_WORKSPACE, "grad_norm: workspace too small");
-    const auto plan = plan_spans(spans_host, n_spans);
-    switch (norm_type) {
-        case XSG_NORM_2: norm_all<2>(plan, sums, slots, norm, norms, as_cuda(stream)); break;
-        case XSG_NORM_1: norm_all<1>(plan, sums, slots, norm, norms, as_cuda(stream)); break;
-        case XSG_NORM_INF: norm_all<kNormInf>(plan, sums, slots, norm, norms, as_cuda(stream)); break;
-        default: return set_error(XSG_ERR_INVALID_ARGUMENT, "grad_norm: unknown norm type");
+    plan.template partials<P>(sums, slots, st);
+    for (size_t l = 0; l < plan.launches.size(); ++l) {
+        const SpanLaunch<N>& L = plan.launches[l];
+        const bool last = l + 1 == plan.launches.size();
+        if (!slots && !last) continue;
+        // the first of these follows the last first pass directly
+        launch_table(norm_finish_kernel<P, N>, 1 + (slots ? L.tab.count : 0), kOptThreads, 1, !slots || l == 0, st,
+                     L.tab, L.blocks, sums, int(plan.sums), slots ? slots + L.slots_at : nullptr,
+                     last ? norm : nullptr, norms ? norms + L.first_span : nullptr);
     }
-    return check_launch("grad_norm");
+    return XSG_OK;
 }
 
-static int clip_grads(const xsg_span* spans_host, int64_t n_spans, int norm_type, float max_norm, float* norm,
-                              void* workspace, size_t workspace_bytes, xsg_stream_t stream) {
-    if (int rc = check_spans(spans_host, n_spans, "clip_grads")) return rc;
+template <int P, int N>
+int clip_all(const SpanPlan<N>& plan, float max_norm, float* norm, Arena arena, int64_t n, cudaStream_t st) {
+    if constexpr (N == kSmallSpans) {
+        if (plan.small(kSmallNormBytes)) {
+            launch_table(clip_small_kernel<P>, plan.cluster(), kSmallThreads, plan.cluster(), false, st,
+                         plan.launches[0].tab, max_norm, norm);
+            return XSG_OK;
+        }
+    }
+    double* sums = arena.take<double>(sums_count(n));
+    if (!sums) return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
+    plan.template partials<P>(sums, nullptr, st);
+    for (size_t l = plan.launches.size(); l-- > 0;)
+        launch_table(clip_scale_kernel<P, N>, plan.launches[l].blocks, kOptThreads, 1, l + 1 == plan.launches.size(),
+                     st, plan.launches[l].tab, sums, int(plan.sums), max_norm, l == 0 ? norm : nullptr);
+    return XSG_OK;
+}
+
+// body(P) for a norm type.
+template <typename F>
+int with_norm_type(int norm_type, const char* what, F&& body) {
+    switch (norm_type) {
+        case XSG_NORM_2: return body(std::integral_constant<int, 2>{});
+        case XSG_NORM_1: return body(std::integral_constant<int, 1>{});
+        case XSG_NORM_INF: return body(std::integral_constant<int, kNormInf>{});
+        default: return set_error(XSG_ERR_INVALID_ARGUMENT, std::string(what) + ": unknown norm type");
+    }
+}
+
+// body(plan) with the table that the number of tensors asks for.
+template <typename Get, typename F>
+int with_plan(int64_t n, Get&& get, F&& body) {
+    if (n <= kSmallSpans) return body(SpanPlan<kSmallSpans>(n, get));
+    return body(SpanPlan<kSpans>(n, get));
+}
+
+int grad_norm(const xsg_span* spans, int64_t n, int norm_type, float* norm, float* norms, Arena arena,
+              cudaStream_t st) {
+    if (int rc = check_spans(spans, n, "grad_norm")) return rc;
+    XSG_REQUIRE(norm, "grad_norm: null output");
+    if (arena.cap < xsg_grad_norm_workspace_size(n)) return set_error(XSG_ERR_WORKSPACE, "grad_norm: workspace too small");
+    const auto get = [&](int64_t i, auto& L) { L.add(spans[i].data, spans[i].n, spans[i].dtype); };
+    const int rc = with_plan(n, get, [&](const auto& plan) {
+        return with_norm_type(norm_type, "grad_norm",
+                              [&](auto p) { return norm_all<decltype(p)::value>(plan, norm, norms, arena, n, st); });
+    });
+    return rc ? rc : check_launch("grad_norm");
+}
+
+int clip_grads(const xsg_span* spans, int64_t n, int norm_type, float max_norm, float* norm, Arena arena,
+               cudaStream_t st) {
+    if (int rc = check_spans(spans, n, "clip_grads")) return rc;
     XSG_REQUIRE(norm, "clip_grads: null output");
     XSG_REQUIRE(max_norm >= 0.f && std::isfinite(max_norm), "clip_grads: max_norm must be finite and not negative");
-    Arena arena(workspace, workspace ? workspace_bytes : 0);
-    double* sums = arena.take<double>(span_launches(n_spans) * kOptBlocks);
-    if (!sums) return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
-    const auto plan = plan_spans(spans_host, n_spans);
-    switch (norm_type) {
-        case XSG_NORM_2: clip_all<2>(plan, sums, max_norm, norm, as_cuda(stream)); break;
-        case XSG_NORM_1: clip_all<1>(plan, sums, max_norm, norm, as_cuda(stream)); break;
-        case XSG_NORM_INF: clip_all<kNormInf>(plan, sums, max_norm, norm, as_cuda(stream)); break;
-        default: return set_error(XSG_ERR_INVALID_ARGUMENT, "clip_grads: unknown norm type");
-    }
-    return check_launch("clip_grads");
+    if (arena.cap < xsg_grad_norm_workspace_size(n)) return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
+    const auto get = [&](int64_t i, auto& L) { L.add(spans[i].data, spans[i].n, spans[i].dtype); };
+    const int rc = with_plan(n, get, [&](const auto& plan) {
+        return with_norm_type(norm_type, "clip_grads",
+                              [&](auto p) { return clip_all<decltype(p)::value>(plan, max_norm, norm, arena, n, st); });
+    });
+    return rc ? rc : check_launch("clip_grads");
 }
 
-static int adamw_update(const xsg_adamw_span* spans_host, int64_t n_spans, int64_t* step, float max_norm,
-                                int skip_nonfinite, float* norm, void* workspace, size_t workspace_bytes,
-                                xsg_stream_t stream) {
-    XSG_REQUIRE(n_spans > 0 && spans_host, "adamw_update: at least one tensor is needed");
-    XSG_REQUIRE(step, "adamw_update: null step counter");
-    XSG_REQUIRE(max_norm < 0.f || std::isfinite(max_norm), "adamw_update: max_norm must be finite");
-    const bool clip = max_norm >= 0.f, normed = clip || skip_nonfinite || norm;
-    std::vector<xsg_span> grads(normed ? n_spans : 0);
+// ---- AdamW
+int check_adamw(const xsg_adamw_span* spans, int64_t n) {
+    XSG_REQUIRE(n > 0 && spans, "adamw_update: at least one tensor is needed");
     int64_t total = 0;
-    for (int64_t i = 0; i < n_spans; ++i) {
-        const xsg_adamw_span& s = spans_host[i];
+    for (int64_t i = 0; i < n; ++i) {
+        const xsg_adamw_span& s = spans[i];
         XSG_REQUIRE(known_dtype(s.param_dtype) && known_dtype(s.grad_dtype), "adamw_update: unknown element type");
         XSG_REQUIRE(s.n >= 0 && s.n < kMaxElems - total, "adamw_update: bad element count");
         total += s.n;
@@ -782,86 +970,177 @@ static int adamw_update(const xsg_adamw_span* spans_host, int64_t n_spans, int64
         XSG_REQUIRE(s.beta1 >= 0 && s.beta1 < 1 && s.beta2 >= 0 && s.beta2 < 1, "adamw_update: betas must be in [0, 1)");
         XSG_REQUIRE(s.eps >= 0 && std::isfinite(s.lr) && std::isfinite(s.weight_decay),
                     "adamw_update: bad learning rate, eps or weight decay");
-        if (normed) grads[i] = {const_cast<void*>(s.grad), s.n, s.grad_dtype};
     }
-    AdamCall call{};
-    call.step = reinterpret_cast<long long*>(step);
-    call.clip = clip;
-    call.skip_nonfinite = skip_nonfinite != 0;
-    call.max_norm = max_norm;
-    if (normed) {
-        Arena arena(workspace, workspace ? workspace_bytes : 0);
-        double* sums = arena.take<double>(span_launches(n_spans) * kOptBlocks);
-        if (!sums) return set_error(XSG_ERR_WORKSPACE, "adamw_update: workspace too small");
-        const auto plan = plan_spans(grads.data(), n_spans);
-        launch_partials<2>(plan, sums, nullptr, as_cuda(stream));
-        call.sums = sums;
-        call.n_sums = total_sums(plan);
-    }
-    AdamTable<kAdamSpans> tab;
-    for (int64_t i = 0; i < n_spans;) {
-        int64_t tiles = 0;
-        int groups = 0, t = 0;
-        bool f32 = true;
-        for (; t < kAdamSpans && i < n_spans; ++t, ++i) {
-            const xsg_adamw_span& s = spans_host[i];
-            AdamHyper h{};
-            h.beta1 = float(s.beta1);
-            h.rest1 = float(1.0 - s.beta1);
-            h.beta2 = float(s.beta2);
-            h.rest2 = float(1.0 - s.beta2);
-            h.lr = float(s.lr);
-            h.lr_decay = float(s.lr * s.weight_decay);
-            h.eps = float(s.eps);
-            h.log_beta1 = float(std::log(s.beta1));
-            h.log_beta2 = float(std::log(s.beta2));
-            int g = 0;
-            while (g < groups && std::memcmp(&tab.hyper[g], &h, sizeof(h)) != 0) ++g;
+    return XSG_OK;
+}
+
+// How far the parameter is past a multiple of 64 elements, or -1 if another
+// array of the update is not as far past a multiple of four.
+int common_lead(const xsg_adamw_span& s) {
+    const auto past = [](const void* p, int size, int of) { return int(reinterpret_cast<uintptr_t>(p) / size % of); };
+    const int lead = past(s.param, elem_size(s.param_dtype), kAdamLine);
+    const bool all = past(s.grad, elem_size(s.grad_dtype), 4) == lead % 4 && past(s.exp_avg, 4, 4) == lead % 4 &&
+                     past(s.exp_avg_sq, 4, 4) == lead % 4 && (!s.master || past(s.master, 4, 4) == lead % 4);
+    return all ? lead : -1;
+}
+
+AdamHyper hyper_of(const xsg_adamw_span& s) {
+    AdamHyper h{};
+    h.beta1 = float(s.beta1);
+    h.rest1 = float(1.0 - s.beta1);
+    h.beta2 = float(s.beta2);
+    h.rest2 = float(1.0 - s.beta2);
+    h.lr = float(s.lr);
+    h.lr_decay = float(s.lr * s.weight_decay);
+    h.eps = float(s.eps);
+    h.log_beta1 = float(std::log(s.beta1));
+    h.log_beta2 = float(std::log(s.beta2));
+    return h;
+}
+
+// Fills a table with tensors from `i` on, as many as it holds (tensors and
+// different groups of options); returns the first that is not in.
+template <int N>
+int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int64_t n, bool& f32) {
+    int groups = 0, t = 0, g = 0;
+    int64_t tiles = 0;
+    f32 = true;
+    for (; t < N && i < n; ++t, ++i) {
+        const xsg_adamw_span& s = spans[i];
+        const auto same = [&](const xsg_adamw_span& o) {
+            return s.lr == o.lr && s.beta1 == o.beta1 && s.beta2 == o.beta2 && s.eps == o.eps &&
+                   s.weight_decay == o.weight_decay;
+        };
+        if (t == 0 || !same(spans[i - 1])) {  // the options of the one before are its own, mostly
+            const AdamHyper h = hyper_of(s);
+            for (g = 0; g < groups && std::memcmp(&tab.hyper[g], &h, sizeof(h)) != 0;) ++g;
             if (g == kAdamGroups) break;
             if (g == groups) tab.hyper[groups++] = h;
-            AdamEntry& e = tab.entry[t];
-            const int lead = common_lead(s);
-            const auto back = [&](void* p, int size) { return static_cast<char*>(p) - std::max(lead, 0) * size; };
-            e.vec = lead >= 0;
-            e.lead = uint8_t(std::max(lead, 0));
-            e.group = uint8_t(g);
-            e.param = back(s.param, elem_size(s.param_dtype));
-            e.grad = back(const_cast<void*>(s.grad), elem_size(s.grad_dtype));
-            e.exp_avg = reinterpret_cast<float*>(back(s.exp_avg, 4));
-            e.exp_avg_sq = reinterpret_cast<float*>(back(s.exp_avg_sq, 4));
-            e.master = s.master ? reinterpret_cast<float*>(back(s.master, 4)) : nullptr;
-            e.rows = s.row_mask;
-            e.end = e.lead + s.n;
-            e.row_size = int32_t(s.row_size);
-            e.param_dtype = uint8_t(s.param_dtype);
-            e.grad_dtype = uint8_t(s.grad_dtype);
-            f32 = f32 && s.param_dtype == XSG_F32 && s.grad_dtype == XSG_F32 && !s.master;
-            tab.first[t] = int32_t(tiles);
-            tiles += s.n ? (e.lead + s.n + kAdamTile - 1) / kAdamTile : 0;
         }
+        AdamEntry& e = tab.entry[t];
+        const int lead = common_lead(s);
+        const auto back = [&](const void* p, int size) {
+            return const_cast<char*>(static_cast<const char*>(p)) - std::max(lead, 0) * size;
+        };
+        e.vec = lead >= 0;
+        e.lead = uint8_t(std::max(lead, 0));
+        e.group = uint8_t(g);
+        e.param = back(s.param, elem_size(s.param_dtype));
+        e.grad = back(s.grad, elem_size(s.grad_dtype));
+        e.exp_avg = reinterpret_cast<float*>(back(s.exp_avg, 4));
+        e.exp_avg_sq = reinterpret_cast<float*>(back(s.exp_avg_sq, 4));
+        e.master = s.master ? reinterpret_cast<float*>(back(s.master, 4)) : nullptr;
+        e.rows = s.row_mask;
+        e.end = e.lead + s.n;
+        e.row_size = int32_t(s.row_size);
+        e.param_dtype = uint8_t(s.param_dtype);
+        e.grad_dtype = uint8_t(s.grad_dtype);
+        f32 = f32 && s.param_dtype == XSG_F32 && s.grad_dtype == XSG_F32 && !s.master;
         tab.first[t] = int32_t(tiles);
-        tab.count = t;
-        const bool last = i >= n_spans;
-        call.advance = last;
-        call.norm = last ? norm : nullptr;
-        const unsigned blocks = unsigned(std::max<int64_t>(1, std::min<int64_t>(tiles, 148 * kAdamResident)));
-        launch(f32 ? adamw_kernel<kAdamSpans, true> : adamw_kernel<kAdamSpans, false>, blocks, kOptThreads, 0,
-               as_cuda(stream), tab, call);
+        tiles += s.n ? (e.lead + s.n + kAdamTile - 1) / kAdamTile : 0;
+    }
+    tab.first[t] = int32_t(tiles);
+    tab.count = t;
+    return i;
+}
+
+template <int N>
+void adamw_all(const xsg_adamw_span* spans, int64_t n, AdamCall call, float* norm, cudaStream_t st) {
+    AdamTable<N> tab;
+    bool pdl = call.sums != nullptr;  // the first launch follows the norm's first pass directly
+    for (int64_t i = 0; i < n;) {
+        bool f32;
+        i = fill_adam(tab, spans, i, n, f32);
+        call.advance = i >= n;
+        call.norm = i >= n ? norm : nullptr;
+        const int blocks = std::max(1, std::min(tab.first[tab.count], 148 * kAdamResident));
+        launch_table(f32 ? adamw_kernel<N, true> : adamw_kernel<N, false>, blocks, kOptThreads, 1, pdl, st, tab, call);
+        pdl = false;
+    }
+}
+
+int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float max_norm, bool skip_nonfinite,
+                 float* norm, Arena arena, cudaStream_t st) {
+    if (int rc = check_adamw(spans, n)) return rc;
+    XSG_REQUIRE(step, "adamw_update: null step counter");
+    XSG_REQUIRE(max_norm < 0.f || std::isfinite(max_norm), "adamw_update: max_norm must be finite");
+    AdamCall call{};
+    call.step = reinterpret_cast<long long*>(step);
+    call.clip = max_norm >= 0.f;
+    call.skip_nonfinite = skip_nonfinite;
+    call.max_norm = max_norm;
+    int rc = XSG_OK;
+    bool done = false;
+    if (call.clip || skip_nonfinite || norm) {
+        if (arena.cap < xsg_grad_norm_workspace_size(n))
+            return set_error(XSG_ERR_WORKSPACE, "adamw_update: workspace too small");
+        const auto get = [&](int64_t i, auto& L) { L.add(spans[i].grad, spans[i].n, spans[i].grad_dtype); };
+        rc = with_plan(n, get, [&](const auto& plan) {
+            const auto& first = plan.launches[0];
+            int64_t elems = 0;
+            for (int64_t i = 0; i < n; ++i) elems += spans[i].n;
+            if constexpr (std::is_same_v<decltype(first.tab), SpanTable<kSmallSpans>>) {
+                if (elems <= kSmallAdamElems) {
+                    AdamTable<kSmallSpans> tab;
+                    bool f32;
+                    fill_adam(tab, spans, 0, n, f32);
+                    call.norm = norm;
+                    launch_table(f32 ? adamw_small_kernel<true> : adamw_small_kernel<false>, plan.cluster(),
+                                 kSmallThreads, plan.cluster(), false, st, first.tab, tab, call);
+                    done = true;
+                    return int(XSG_OK);
+                }
+            }
+            double* sums = arena.take<double>(sums_count(n));
+            plan.template partials<2>(sums, nullptr, st);
+            call.sums = sums;
+            call.n_sums = int(plan.sums);
+            return int(XSG_OK);
+        });
+    }
+    if (rc) return rc;
+    if (!done) {
+        if (n <= kSmallSpans) adamw_all<kSmallSpans>(spans, n, call, norm, st);
+        else adamw_all<kAdamSpans>(spans, n, call, norm, st);
     }
     return check_launch("adamw_update");
+}
+
+// No C++ exception leaves a C entry.
+template <typename F>
+int guarded(const char* what, F&& body) {
+    try {
+        return body();
+    } catch (const std::exception& e) {
+        return set_error(XSG_ERR_INVALID_ARGUMENT, std::string(what) + ": " + e.what());
+    }
+}
+
+Arena arena_of(void* workspace, size_t bytes) { return Arena(workspace, workspace ? bytes : 0); }
+
+}  // namespace
+}  // namespace xsg
+
+using namespace xsg;
+
+extern "C" size_t xsg_grad_norm_workspace_size(int64_t n_spans) {
+    if (n_spans <= 0) return 0;
+    return Arena::round(sums_count(n_spans) * sizeof(double)) + Arena::round(slots_count(n_spans) * sizeof(double));
 }
 
 extern "C" int xsg_grad_norm(const xsg_span* spans_host, int64_t n_spans, int norm_type, float* norm, float* norms,
                              void* workspace, size_t workspace_bytes, xsg_stream_t stream) {
     return guarded("grad_norm", [&] {
-        return grad_norm(spans_host, n_spans, norm_type, norm, norms, workspace, workspace_bytes, stream);
+        return grad_norm(spans_host, n_spans, norm_type, norm, norms, arena_of(workspace, workspace_bytes),
+                         as_cuda(stream));
     });
 }
 
 extern "C" int xsg_clip_grads(const xsg_span* spans_host, int64_t n_spans, int norm_type, float max_norm, float* norm,
                               void* workspace, size_t workspace_bytes, xsg_stream_t stream) {
     return guarded("clip_grads", [&] {
-        return clip_grads(spans_host, n_spans, norm_type, max_norm, norm, workspace, workspace_bytes, stream);
+        return clip_grads(spans_host, n_spans, norm_type, max_norm, norm, arena_of(workspace, workspace_bytes),
+                          as_cuda(stream));
     });
 }
 
@@ -869,7 +1148,7 @@ extern "C" int xsg_adamw_update(const xsg_adamw_span* spans_host, int64_t n_span
                                 int skip_nonfinite, float* norm, void* workspace, size_t workspace_bytes,
                                 xsg_stream_t stream) {
     return guarded("adamw_update", [&] {
-        return adamw_update(spans_host, n_spans, step, max_norm, skip_nonfinite, norm, workspace, workspace_bytes,
-                            stream);
+        return adamw_update(spans_host, n_spans, step, max_norm, skip_nonfinite != 0, norm,
+                            arena_of(workspace, workspace_bytes), as_cuda(stream));
     });
 }
