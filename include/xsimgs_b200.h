@@ -547,8 +547,10 @@ typedef struct xsg_span {
     int64_t n;     /* elements */
     int32_t dtype; /* xsg_dtype */
 } xsg_span;
-/* Scratch of the three calls below. */
+/* Scratch of the three calls below: enough for any tensors, or for these
+ * (0 where one launch does without). */
 size_t xsg_grad_norm_workspace_size(int64_t n_spans);
+size_t xsg_grad_norm_workspace_bytes(const xsg_span* spans_host, int64_t n_spans);
 /* norm [1] = the norm of all elements of all tensors; norms [n_spans] (may be
  * NULL) = each tensor's.  NaN and infinite elements give a NaN or infinite
  * norm. */
@@ -576,6 +578,7 @@ typedef struct xsg_adamw_span {
     int32_t grad_dtype;
     double lr, beta1, beta2, eps, weight_decay;
 } xsg_adamw_span;
+size_t xsg_adamw_workspace_bytes(const xsg_adamw_span* spans_host, int64_t n_spans);
 /* step [2]: the number of updates taken so far, which the call advances by
  * one, and a word that is zero between calls.  With t = step + 1:
  *   g' = c g, m <- b1 m + (1 - b1) g', v <- b2 v + (1 - b2) g'^2,

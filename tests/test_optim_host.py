@@ -30,6 +30,13 @@ def test_workspace_size(lib):
     size = lib.xsg_grad_norm_workspace_size
     assert size(0) == 0 and size(-3) == 0
     assert 0 < size(1) <= size(1000) <= size(5000) < 1 << 20
+    lib.xsg_grad_norm_workspace_bytes.restype = lib.xsg_adamw_workspace_bytes.restype = C.c_size_t
+    for n, need in ((8, 0), (1 << 22, size(1))):
+        assert lib.xsg_grad_norm_workspace_bytes((Span * 1)(Span(None, n, 0)), C.c_int64(1)) == need
+        assert lib.xsg_adamw_workspace_bytes((AdamSpan * 1)(AdamSpan(n=n)), C.c_int64(1)) == need
+    many = (Span * 40)(*[Span(None, 1, 0)] * 40)
+    assert lib.xsg_grad_norm_workspace_bytes(many, C.c_int64(40)) == size(40)
+    assert lib.xsg_grad_norm_workspace_bytes(None, C.c_int64(40)) == 0
 
 
 def refuse(lib, rc, code, text):
@@ -47,8 +54,9 @@ def test_c_abi_refusals(lib):
     refuse(lib, norm(spans=None), 1, b"at least one tensor")
     refuse(lib, norm(out=None), 1, b"null output")
     refuse(lib, norm(p=3), 1, b"norm type")
-    refuse(lib, norm(ws=None), 4, b"workspace")
-    refuse(lib, norm(size=8), 4, b"workspace")
+    large = (Span * 1)(Span(fake, 1 << 22, 0))  # small ones go in one launch, without scratch
+    refuse(lib, norm(spans=large, ws=None), 4, b"workspace")
+    refuse(lib, norm(spans=large, size=8), 4, b"workspace")
     refuse(lib, norm(spans=(Span * 1)(Span(fake, -1, 0))), 1, b"element count")
     refuse(lib, norm(spans=(Span * 1)(Span(fake, 1 << 40, 0))), 1, b"element count")
     refuse(lib, norm(spans=(Span * 1)(Span(None, 4, 0))), 1, b"null pointer")
@@ -81,7 +89,7 @@ def test_c_abi_refusals(lib):
     refuse(lib, adamw(eps=-1.0), 1, b"eps")
     refuse(lib, adamw(lr=float("nan")), 1, b"learning rate")
     refuse(lib, adamw(max_norm=float("inf")), 1, b"max_norm")
-    refuse(lib, adamw(max_norm=1.0, ws=None), 4, b"workspace")
+    refuse(lib, adamw(n=1 << 22, max_norm=1.0, ws=None), 4, b"workspace")
 
 
 def test_extension_refusals_without_gpu():
@@ -102,6 +110,10 @@ def test_extension_refusals_without_gpu():
         (lambda: X.adamw_update_([t], [t], [t], [t], step, lr=[0.1, 0.2, 0.3]), "one value"),
     ]:
         with pytest.raises(RuntimeError, match=match):
+            call()
+    for call in (lambda: X.gradient_norm([1.0]), lambda: X.gradient_norm(3), lambda: X.clip_gradients_([None], 1.0),
+                 lambda: X.adamw_update_([t], [t], [t], [t], step, lr="fast")):
+        with pytest.raises(TypeError):
             call()
 
 

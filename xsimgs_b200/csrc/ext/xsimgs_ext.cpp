@@ -918,6 +918,54 @@ std::tuple<Tensor, Tensor, Tensor> interpolate_smpl_bwd(const Tensor& poses, con
 }
 
 // ------------------------------------------- the end of a training step --
+// The tensors of a Python sequence, borrowed: a call over hundreds of tensors
+// spends its host time here.
+struct TensorList {
+    py::object seq;  // a list or a tuple
+    std::vector<const Tensor*> at;
+
+    TensorList(const py::object& o, const char* name, bool optional = false) {
+        seq = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), name));
+        if (!seq) throw py::error_already_set();
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq.ptr());
+        at.reserve(size_t(n));
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            PyObject* x = PySequence_Fast_GET_ITEM(seq.ptr(), i);
+            if (optional && x == Py_None) {
+                at.push_back(nullptr);
+                continue;
+            }
+            TORCH_CHECK_TYPE(THPVariable_Check(x), name, " must be tensors, got ", Py_TYPE(x)->tp_name);
+            at.push_back(&THPVariable_Unpack(x));
+        }
+    }
+    size_t size() const { return at.size(); }
+    bool empty() const { return at.empty(); }
+    const Tensor& operator[](size_t i) const { return *at[i]; }
+};
+
+// One number for all tensors, or one for each.
+struct Numbers {
+    std::vector<double> v;
+
+    Numbers(const py::object& o, size_t n, const char* name) {
+        if (PyList_Check(o.ptr()) || PyTuple_Check(o.ptr())) {
+            const Py_ssize_t m = PySequence_Fast_GET_SIZE(o.ptr());
+            v.reserve(size_t(m));
+            for (Py_ssize_t i = 0; i < m; ++i) v.push_back(number(PySequence_Fast_GET_ITEM(o.ptr(), i)));
+            TORCH_CHECK(v.size() == n, "adamw_update_: ", name, " must be one value or one for each param");
+        } else {
+            v.push_back(number(o.ptr()));
+        }
+    }
+    static double number(PyObject* x) {
+        const double d = PyFloat_AsDouble(x);
+        if (d == -1.0 && PyErr_Occurred()) throw py::error_already_set();
+        return d;
+    }
+    double operator[](size_t i) const { return v.size() == 1 ? v[0] : v[i]; }
+};
+
 int dtype_code(const Tensor& t, const char* name) {
     switch (t.scalar_type()) {
         case at::kFloat: return XSG_F32;
@@ -980,7 +1028,19 @@ int norm_code(double p) {
     return XSG_NORM_INF;
 }
 
-py::object gradient_norm(const std::vector<Tensor>& grads, double norm_type, bool per_tensor) {
+// Scratch of a norm; none where one launch does without.
+struct NormScratch {
+    Tensor t;
+    size_t bytes;
+    NormScratch(const std::vector<xsg_span>& spans, const Tensor& like)
+        : bytes(xsg_grad_norm_workspace_bytes(spans.data(), int64_t(spans.size()))) {
+        if (bytes) t = workspace(bytes, like);
+    }
+    void* data() const { return bytes ? t.data_ptr() : nullptr; }
+};
+
+py::object gradient_norm(const py::object& grads_seq, double norm_type, bool per_tensor) {
+    const TensorList grads(grads_seq, "grads");
     TORCH_CHECK(!grads.empty(), "gradient_norm: at least one tensor is needed");
     const int p = norm_code(norm_type);
     std::vector<Tensor> copies;  // of tensors with gaps or expanded dimensions
@@ -998,14 +1058,15 @@ py::object gradient_norm(const std::vector<Tensor>& grads, double norm_type, boo
     const auto f32 = grads[0].options().dtype(at::kFloat).requires_grad(false);
     Tensor norm = at::empty({}, f32);
     Tensor norms = per_tensor ? at::empty({int64_t(grads.size())}, f32) : Tensor();
-    Tensor ws = workspace(xsg_grad_norm_workspace_size(int64_t(spans.size())), norm);
+    const NormScratch ws(spans, norm);
     check(xsg_grad_norm(spans.data(), int64_t(spans.size()), p, fptr_mut(norm), per_tensor ? fptr_mut(norms) : nullptr,
-                        ws.data_ptr(), size_t(ws.nbytes()), stream()));
+                        ws.data(), ws.bytes, stream()));
     if (per_tensor) return py::make_tuple(norm, norms);
     return py::cast(norm);
 }
 
-Tensor clip_gradients(const std::vector<Tensor>& grads, double max_norm, double norm_type) {
+Tensor clip_gradients(const py::object& grads_seq, double max_norm, double norm_type) {
+    const TensorList grads(grads_seq, "grads");
     TORCH_CHECK(!grads.empty(), "clip_gradients_: at least one tensor is needed");
     const int p = norm_code(norm_type);
     TORCH_CHECK(std::isfinite(max_norm) && max_norm >= 0.0 && max_norm <= std::numeric_limits<float>::max(),
@@ -1021,33 +1082,33 @@ Tensor clip_gradients(const std::vector<Tensor>& grads, double max_norm, double 
     check_apart(extents, "clip_gradients_");
     c10::cuda::CUDAGuard g(grads[0].device());
     Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
-    Tensor ws = workspace(xsg_grad_norm_workspace_size(int64_t(spans.size())), norm);
-    for (const Tensor& t : grads) torch::autograd::impl::bump_version(t);
-    check(xsg_clip_grads(spans.data(), int64_t(spans.size()), p, float(max_norm), fptr_mut(norm), ws.data_ptr(),
-                         size_t(ws.nbytes()), stream()));
+    const NormScratch ws(spans, norm);
+    for (size_t i = 0; i < grads.size(); ++i) torch::autograd::impl::bump_version(grads[i]);
+    check(xsg_clip_grads(spans.data(), int64_t(spans.size()), p, float(max_norm), fptr_mut(norm), ws.data(), ws.bytes,
+                         stream()));
     return norm;
 }
 
-// One value for all tensors, or one for each.
-double nth(const std::vector<double>& v, size_t i) { return v.size() == 1 ? v[0] : v[i]; }
-
-std::optional<Tensor> adamw_update(const std::vector<Tensor>& params, const std::vector<Tensor>& grads,
-                                   const std::vector<Tensor>& exp_avgs, const std::vector<Tensor>& exp_avg_sqs,
-                                   const Tensor& step, const std::vector<double>& lr, const std::vector<double>& beta1,
-                                   const std::vector<double>& beta2, const std::vector<double>& eps,
-                                   const std::vector<double>& weight_decay, std::optional<double> max_norm,
-                                   bool skip_nonfinite, const std::vector<OptT>& masters,
-                                   const std::vector<OptT>& row_masks) {
+std::optional<Tensor> adamw_update(const py::object& params_seq, const py::object& grads_seq,
+                                   const py::object& exp_avgs_seq, const py::object& exp_avg_sqs_seq,
+                                   const Tensor& step, const py::object& lr_values, const py::object& beta1_values,
+                                   const py::object& beta2_values, const py::object& eps_values,
+                                   const py::object& decay_values, std::optional<double> max_norm, bool skip_nonfinite,
+                                   const py::object& masters_seq, const py::object& row_mask) {
+    const TensorList params(params_seq, "params"), grads(grads_seq, "grads"), exp_avgs(exp_avgs_seq, "exp_avgs"),
+        exp_avg_sqs(exp_avg_sqs_seq, "exp_avg_sqs");
     const size_t n = params.size();
     TORCH_CHECK(n > 0, "adamw_update_: at least one tensor is needed");
     TORCH_CHECK(grads.size() == n && exp_avgs.size() == n && exp_avg_sqs.size() == n,
                 "adamw_update_: params, grads, exp_avgs and exp_avg_sqs must have the same length");
-    TORCH_CHECK((masters.empty() || masters.size() == n), "adamw_update_: masters must have one entry for each param");
-    TORCH_CHECK(row_masks.size() <= 1 || row_masks.size() == n,
-                "adamw_update_: row_mask must be one mask or one entry for each param");
-    for (const auto* v : {&lr, &beta1, &beta2, &eps, &weight_decay})
-        TORCH_CHECK(v->size() == 1 || v->size() == n,
-                    "adamw_update_: lr, betas, eps and weight_decay must be one value or one for each param");
+    std::optional<TensorList> masters, masks;
+    if (!masters_seq.is_none()) masters.emplace(masters_seq, "masters", true);
+    TORCH_CHECK(!masters || masters->size() == n, "adamw_update_: masters must have one entry for each param");
+    const Tensor* one_mask = THPVariable_Check(row_mask.ptr()) ? &THPVariable_Unpack(row_mask.ptr()) : nullptr;
+    if (!row_mask.is_none() && !one_mask) masks.emplace(row_mask, "row_mask", true);
+    TORCH_CHECK(!masks || masks->size() == n, "adamw_update_: row_mask must be one mask or one entry for each param");
+    const Numbers lr(lr_values, n, "lr"), beta1(beta1_values, n, "betas"), beta2(beta2_values, n, "betas"),
+        eps(eps_values, n, "eps"), weight_decay(decay_values, n, "weight_decay");
     TORCH_CHECK(!max_norm || (std::isfinite(*max_norm) && *max_norm >= 0.0 &&
                               *max_norm <= std::numeric_limits<float>::max()),
                 "adamw_update_: max_norm must be finite and not negative");
@@ -1065,8 +1126,8 @@ std::optional<Tensor> adamw_update(const std::vector<Tensor>& params, const std:
         const Tensor& p = params[i];
         xsg_adamw_span& s = spans[i];
         check_written(p, "params", params[0]);
-        const bool has_master = !masters.empty() && has(masters[i]);
-        const Tensor* state[3] = {&exp_avgs[i], &exp_avg_sqs[i], has_master ? &*masters[i] : nullptr};
+        const Tensor* master = masters ? masters->at[i] : nullptr;
+        const Tensor* state[3] = {&exp_avgs[i], &exp_avg_sqs[i], master};
         const char* names[3] = {"exp_avgs", "exp_avg_sqs", "masters"};
         for (int k = 0; k < 3; ++k) {
             if (!state[k]) continue;
@@ -1090,49 +1151,48 @@ std::optional<Tensor> adamw_update(const std::vector<Tensor>& params, const std:
         s.grad = grad.data_ptr();
         s.exp_avg = fptr_mut(exp_avgs[i]);
         s.exp_avg_sq = fptr_mut(exp_avg_sqs[i]);
-        s.master = has_master ? fptr_mut(*masters[i]) : nullptr;
+        s.master = master ? fptr_mut(*master) : nullptr;
         s.n = p.numel();
         s.row_size = 0;
         s.row_mask = nullptr;
-        if (!row_masks.empty()) {
-            const OptT& mask = row_masks.size() == 1 ? row_masks[0] : row_masks[i];
-            if (has(mask)) {
-                check_listed(*mask, "row_mask", params[0]);
-                TORCH_CHECK(mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte,
-                            "row_mask must be bool or uint8");
-                TORCH_CHECK(mask->dim() == 1 && mask->is_contiguous(), "row_mask must be one contiguous dimension");
-                TORCH_CHECK(p.dim() >= 1 && p.size(0) == mask->size(0), "row_mask must have one entry for each of the ",
-                            p.dim() >= 1 ? p.size(0) : 0, " rows of its parameter, got ", mask->size(0));
-                TORCH_CHECK(p.is_contiguous(), "params under a row_mask must be contiguous");
-                if (s.n > 0) {
-                    s.row_mask = static_cast<const uint8_t*>(mask->data_ptr());
-                    s.row_size = s.n / p.size(0);
-                    TORCH_CHECK(s.row_size < (int64_t(1) << 30), "adamw_update_: rows under a mask are too long");
-                }
+        if (const Tensor* mask = masks ? masks->at[i] : one_mask) {
+            check_listed(*mask, "row_mask", params[0]);
+            TORCH_CHECK(mask->scalar_type() == at::kBool || mask->scalar_type() == at::kByte,
+                        "row_mask must be bool or uint8");
+            TORCH_CHECK(mask->dim() == 1 && mask->is_contiguous(), "row_mask must be one contiguous dimension");
+            TORCH_CHECK(p.dim() >= 1 && p.size(0) == mask->size(0), "row_mask must have one entry for each of the ",
+                        p.dim() >= 1 ? p.size(0) : 0, " rows of its parameter, got ", mask->size(0));
+            TORCH_CHECK(p.is_contiguous(), "params under a row_mask must be contiguous");
+            if (s.n > 0) {
+                s.row_mask = static_cast<const uint8_t*>(mask->data_ptr());
+                s.row_size = s.n / p.size(0);
+                TORCH_CHECK(s.row_size < (int64_t(1) << 30), "adamw_update_: rows under a mask are too long");
             }
         }
-        s.lr = nth(lr, i);
-        s.beta1 = nth(beta1, i);
-        s.beta2 = nth(beta2, i);
-        s.eps = nth(eps, i);
-        s.weight_decay = nth(weight_decay, i);
+        s.lr = lr[i];
+        s.beta1 = beta1[i];
+        s.beta2 = beta2[i];
+        s.eps = eps[i];
+        s.weight_decay = weight_decay[i];
     }
     check_apart(extents, "adamw_update_");
     const bool normed = max_norm.has_value() || skip_nonfinite;
     Tensor norm, ws;
+    size_t bytes = 0;
     if (normed) {
         norm = at::empty({}, params[0].options().dtype(at::kFloat).requires_grad(false));
-        ws = workspace(xsg_grad_norm_workspace_size(int64_t(n)), norm);
+        bytes = xsg_adamw_workspace_bytes(spans.data(), int64_t(n));
+        if (bytes) ws = workspace(bytes, norm);
     }
     for (size_t i = 0; i < n; ++i) {
         torch::autograd::impl::bump_version(params[i]);
         torch::autograd::impl::bump_version(exp_avgs[i]);
         torch::autograd::impl::bump_version(exp_avg_sqs[i]);
-        if (spans[i].master) torch::autograd::impl::bump_version(*masters[i]);
+        if (spans[i].master) torch::autograd::impl::bump_version((*masters)[i]);
     }
     check(xsg_adamw_update(spans.data(), int64_t(n), step.data_ptr<int64_t>(), max_norm ? float(*max_norm) : -1.f,
-                           skip_nonfinite, normed ? fptr_mut(norm) : nullptr, normed ? ws.data_ptr() : nullptr,
-                           normed ? size_t(ws.nbytes()) : 0, stream()));
+                           skip_nonfinite, normed ? fptr_mut(norm) : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
+                           stream()));
     return normed ? std::optional<Tensor>(norm) : std::nullopt;
 }
 
@@ -1332,5 +1392,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adamw_update_", &adamw_update, py::arg("params"), py::arg("grads"), py::arg("exp_avgs"),
           py::arg("exp_avg_sqs"), py::arg("step"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
           py::arg("weight_decay"), py::arg("max_norm") = py::none(), py::arg("skip_nonfinite") = false,
-          py::arg("masters") = std::vector<OptT>{}, py::arg("row_masks") = std::vector<OptT>{});
+          py::arg("masters") = py::none(), py::arg("row_mask") = py::none());
 }

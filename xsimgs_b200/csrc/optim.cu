@@ -61,7 +61,6 @@ __device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float x)
 // five lines for four, and two warps write parts of one).  Tile k holds
 // the numbers [k * tile, (k + 1) * tile); tensor t of a table owns the tiles
 // [first[t], first[t + 1]) of the launch.
-constexpr int kTileBytes = 16384;
 constexpr int kLine = 128;
 
 template <int N>
@@ -72,6 +71,7 @@ struct SpanTable {
     uint8_t lead[N];
     uint8_t dtype[N];
     int32_t count;
+    int32_t tile_bytes;
 };
 
 // The part of tensor t in the tiles [tile, stop): numbers [lo, hi).
@@ -80,7 +80,7 @@ struct Part {
 };
 template <typename Table>
 __device__ __forceinline__ Part part_of(const Table& tab, int t, int32_t tile, int32_t stop) {
-    const int64_t per = kTileBytes / elem_size(tab.dtype[t]);
+    const int64_t per = tab.tile_bytes / elem_size(tab.dtype[t]);
     return {max(int64_t(tab.lead[t]), (tile - tab.first[t]) * per), min(tab.end[t], (stop - tab.first[t]) * per)};
 }
 
@@ -151,9 +151,10 @@ __device__ __forceinline__ void add16(double& acc, const float (&x)[16]) {
     for (int i = 0; i < 16; ++i) acc += term<P>(x[i]);
 }
 
-// Sum (or maximum) over the numbers [lo, hi) of a tensor, by the block.
+// Sum (or maximum) over the numbers [lo, hi) of a tensor, by a team of T
+// threads (a block or a warp) of which this is number `me`.
 template <int P, int D, int T>
-__device__ __forceinline__ double reduce_part(const void* base, Part part) {
+__device__ __forceinline__ double reduce_part(const void* base, Part part, int me) {
     constexpr int V = 16 / elem_size(D);  // elements of a vector
     constexpr int kUnroll = 4;
     constexpr int L = kLine / elem_size(D);
@@ -195,7 +196,7 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part) {
             }
         }
     };
-    int i = threadIdx.x;
+    int i = me;
     for (; i + (kUnroll - 1) * T < n; i += kUnroll * T) {
         uint4 q[kUnroll];
 #pragma unroll
@@ -215,17 +216,19 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part) {
     }
     // the elements before the first and after the last of these vectors, each fewer than a line's
     const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
-    const int64_t odd = threadIdx.x < L ? part.lo + threadIdx.x : tail + threadIdx.x - L;
-    if (threadIdx.x < 2 * L && odd < (threadIdx.x < L ? head : part.hi))
-        acc = join<P>(acc, term<P>(load_as(base, D, odd)));
+    for (int j = me; j < 2 * L; j += T) {
+        const int64_t odd = j < L ? part.lo + j : tail + j - L;
+        if (odd < (j < L ? head : part.hi)) acc = join<P>(acc, term<P>(load_as(base, D, odd)));
+    }
     return acc;
 }
 
-template <int P, int T>
-__device__ __forceinline__ double reduce_part(const void* base, int dtype, Part part) {
-    if (dtype == XSG_F32) return reduce_part<P, XSG_F32, T>(base, part);
-    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16, T>(base, part);
-    return reduce_part<P, XSG_F16, T>(base, part);
+template <int P, int T, typename Table>
+__device__ __forceinline__ double reduce_part(const Table& tab, int t, Part part, int me) {
+    const int dtype = tab.dtype[t];
+    if (dtype == XSG_F32) return reduce_part<P, XSG_F32, T>(tab.base[t], part, me);
+    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16, T>(tab.base[t], part, me);
+    return reduce_part<P, XSG_F16, T>(tab.base[t], part, me);
 }
 
 // Over the block, in a fixed order; every thread gets the result.  `smem`
@@ -267,7 +270,7 @@ __global__ void __launch_bounds__(kOptThreads, kOptResident)
     for (int32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         if (t < 0) t = owner_of(tab, tile);
         while (tile >= tab.first[t + 1]) ++t;
-        acc = join<P>(acc, reduce_part<P, kOptThreads>(tab.base[t], tab.dtype[t], part_of(tab, t, tile, tile + 1)));
+        acc = join<P>(acc, reduce_part<P, kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), threadIdx.x));
     }
     acc = block_reduce<P>(acc, smem);
     if (threadIdx.x == 0) sums[blockIdx.x] = acc;
@@ -289,11 +292,13 @@ __global__ void __launch_bounds__(kOptThreads, kOptResident)
     for (int t = owner_of(tab, tile); tile < end; ++t) {
         const int32_t stop = min(end, tab.first[t + 1]);
         if (stop <= tile) continue;
-        const double acc = block_reduce<P>(
-            reduce_part<P, kOptThreads>(tab.base[t], tab.dtype[t], part_of(tab, t, tile, stop)), smem);
+        // tile by tile, so that the same entries meet in 32 bits as in the kernel above
+        double acc = 0.0;
+        for (; tile < stop; ++tile)
+            acc = join<P>(acc, reduce_part<P, kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), threadIdx.x));
+        acc = block_reduce<P>(acc, smem);
         if (threadIdx.x == 0) slots[blockIdx.x + t] = acc;
         whole = join<P>(whole, acc);
-        tile = stop;
     }
     if (threadIdx.x == 0) sums[blockIdx.x] = whole;
 }
@@ -331,8 +336,8 @@ __global__ void __launch_bounds__(kOptThreads)
     if (threadIdx.x == 0) norms[t] = v;
 }
 
-// g <- c g over the numbers [lo, hi) of a tensor, by the block, from the end
-// to the start.  The product is taken in 32 bits and rounded once to g's type.
+// g <- c g over the numbers [lo, hi) of a tensor, by a team of T threads, from
+// the end to the start.  The product is taken in 32 bits and rounded once to g's type.
 template <int D>
 __device__ __forceinline__ uint32_t scaled(uint32_t w, float c) {
     if constexpr (D == XSG_F32) return __float_as_uint(__uint_as_float(w) * c);
@@ -349,14 +354,14 @@ __device__ __forceinline__ uint32_t scaled(uint32_t w, float c) {
 }
 
 template <int D, int T>
-__device__ __forceinline__ void scale_part(void* base, Part part, float c) {
+__device__ __forceinline__ void scale_part(void* base, Part part, float c, int me) {
     constexpr int V = 16 / elem_size(D);
     constexpr int kUnroll = 4, kStep = kUnroll * T;
     constexpr int L = kLine / elem_size(D);
     const int64_t first = (part.lo + L - 1) / L * (L / V), last = part.hi / V;
     uint4* vec = static_cast<uint4*>(base) + first;
     const int n = int(max(last - first, int64_t(0)));  // a block's part is below 2^31 vectors
-    int i = n / kStep * kStep + threadIdx.x;
+    int i = n / kStep * kStep + me;
     for (int j = i; j < n; j += T) {
         const uint4 q = vec[j];
         vec[j] = make_uint4(scaled<D>(q.x, c), scaled<D>(q.y, c), scaled<D>(q.z, c), scaled<D>(q.w, c));
@@ -371,17 +376,18 @@ __device__ __forceinline__ void scale_part(void* base, Part part, float c) {
                 make_uint4(scaled<D>(q[k].x, c), scaled<D>(q[k].y, c), scaled<D>(q[k].z, c), scaled<D>(q[k].w, c));
     }
     const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
-    const int64_t odd = threadIdx.x < L ? part.lo + threadIdx.x : tail + threadIdx.x - L;
-    if (threadIdx.x < 2 * L && odd < (threadIdx.x < L ? head : part.hi))
-        store_as(base, D, odd, load_as(base, D, odd) * c);
+    for (int j = me; j < 2 * L; j += T) {
+        const int64_t odd = j < L ? part.lo + j : tail + j - L;
+        if (odd < (j < L ? head : part.hi)) store_as(base, D, odd, load_as(base, D, odd) * c);
+    }
 }
 
 template <int T, typename Table>
-__device__ __forceinline__ void scale_part(const Table& tab, int t, Part part, float c) {
+__device__ __forceinline__ void scale_part(const Table& tab, int t, Part part, float c, int me) {
     const int dtype = tab.dtype[t];
-    if (dtype == XSG_F32) scale_part<XSG_F32, T>(tab.base[t], part, c);
-    else if (dtype == XSG_BF16) scale_part<XSG_BF16, T>(tab.base[t], part, c);
-    else scale_part<XSG_F16, T>(tab.base[t], part, c);
+    if (dtype == XSG_F32) scale_part<XSG_F32, T>(tab.base[t], part, c, me);
+    else if (dtype == XSG_BF16) scale_part<XSG_BF16, T>(tab.base[t], part, c, me);
+    else scale_part<XSG_F16, T>(tab.base[t], part, c, me);
 }
 
 // The second pass of clipping.  c = 1 leaves the data alone.  The tiles are
@@ -401,24 +407,47 @@ __global__ void __launch_bounds__(kOptThreads, kOptResident)
     for (int32_t tile = tab.first[tab.count] - 1 - int32_t(blockIdx.x); tile >= 0; tile -= gridDim.x) {
         if (t < 0) t = owner_of(tab, tile);
         while (tile < tab.first[t]) --t;
-        scale_part<kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), c);
+        scale_part<kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), c, threadIdx.x);
     }
 }
 
 // --------------------------------------------------------- small tensors --
-// What eight SMs read in a few microseconds goes in one launch: a cluster of
-// blocks, each with a run of the tiles; the blocks' sums meet in shared
-// memory over the cluster, and each block scales what it has just read.
+// What a few SMs read in one round of loads goes in one launch: a cluster of
+// blocks whose warps each take small tiles, so that all loads are under way
+// at once; the blocks' sums meet over the cluster's shared memory.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallBlocks = 8;
 constexpr int kSmallSpans = 32;
+constexpr int kSmallTile = 2048;  // bytes: four vectors a lane
 
 // A block's sums, where the others of the cluster read them.
 struct ClusterSums {
     double whole;
     double each[kSmallSpans];
-    double smem[33];
+    double warp[33];
 };
+
+// This warp among the cluster's.
+struct Worker {
+    int id, count, lane;
+};
+__device__ __forceinline__ Worker worker_of(const cg::cluster_group& cluster) {
+    const int warps = int(blockDim.x >> 5);
+    return {int(cluster.block_rank()) * warps + int(threadIdx.x >> 5), int(cluster.num_blocks()) * warps,
+            int(threadIdx.x & 31)};
+}
+
+// body(t, tile) for the tiles of a worker, in turn.
+template <typename Table, typename F>
+__device__ __forceinline__ void for_tiles(const Table& tab, int32_t first, int32_t step, F&& body) {
+    const int32_t tiles = tab.first[tab.count];
+    int t = -1;
+    for (int32_t tile = first; tile < tiles; tile += step) {
+        if (t < 0) t = owner_of(tab, tile);
+        while (tile >= tab.first[t + 1]) ++t;
+        body(t, tile);
+    }
+}
 
 // Over the cluster, in the order of the ranks; every thread gets it.
 template <int P>
@@ -428,49 +457,66 @@ __device__ __forceinline__ double cluster_join(cg::cluster_group& cluster, doubl
     return v;
 }
 
-// The sum over this block's run of tiles.
-template <int P, bool kEach>
-__device__ __forceinline__ void run_sums(const SpanTable<kSmallSpans>& tab, int32_t rank, int32_t ranks,
-                                         ClusterSums& s) {
-    const int32_t tiles = tab.first[tab.count], end = run_start(tiles, ranks, rank + 1);
-    int32_t tile = run_start(tiles, ranks, rank);
-    if (kEach) {
-        if (threadIdx.x < kSmallSpans) s.each[threadIdx.x] = 0.0;
-        __syncthreads();
-    }
-    double acc = 0.0, whole = 0.0;
-    for (int t = owner_of(tab, tile); tile < end; ++t) {
-        const int32_t stop = min(end, tab.first[t + 1]);
-        if (stop <= tile) continue;
-        acc = join<P>(acc, reduce_part<P, kSmallThreads>(tab.base[t], tab.dtype[t], part_of(tab, t, tile, stop)));
-        if (kEach) {
-            acc = block_reduce<P>(acc, s.smem);
-            if (threadIdx.x == 0) s.each[t] = acc;
-            whole = join<P>(whole, acc);
-            acc = 0.0;
-        }
-        tile = stop;
-    }
-    if (!kEach) whole = block_reduce<P>(acc, s.smem);
-    if (threadIdx.x == 0) s.whole = whole;
+// The norm of all tensors, for every thread of the cluster.
+template <int P>
+__device__ __forceinline__ float cluster_norm(const SpanTable<kSmallSpans>& tab, cg::cluster_group& cluster,
+                                              ClusterSums& sums) {
+    const Worker w = worker_of(cluster);
+    double acc = 0.0;
+    for_tiles(tab, w.id, w.count, [&](int t, int32_t tile) {
+        acc = join<P>(acc, reduce_part<P, 32>(tab, t, part_of(tab, t, tile, tile + 1), w.lane));
+    });
+    acc = block_reduce<P>(acc, sums.warp);
+    if (cluster.num_blocks() == 1) return root<P>(acc);
+    if (threadIdx.x == 0) sums.whole = acc;
+    cluster.sync();
+    const float total = root<P>(cluster_join<P>(cluster, &sums.whole));
+    cluster.sync();  // the others' sums stay until all have read them
+    return total;
 }
 
 template <int P>
 __global__ void __launch_bounds__(kSmallThreads)
-    norm_small_kernel(const __grid_constant__ SpanTable<kSmallSpans> tab, float* __restrict__ norm,
-                      float* __restrict__ norms) {
+    norm_small_kernel(const __grid_constant__ SpanTable<kSmallSpans> tab, float* __restrict__ norm) {
     __shared__ ClusterSums sums;
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = int(cluster.block_rank());
-    if (norms) run_sums<P, true>(tab, rank, int(cluster.num_blocks()), sums);
-    else run_sums<P, false>(tab, rank, int(cluster.num_blocks()), sums);
-    cluster.sync();
-    if (rank == 0) {
-        if (threadIdx.x == 0) *norm = root<P>(cluster_join<P>(cluster, &sums.whole));
-        if (norms && int(threadIdx.x) >= 32 && int(threadIdx.x) < 32 + tab.count)
-            norms[threadIdx.x - 32] = root<P>(cluster_join<P>(cluster, &sums.each[threadIdx.x - 32]));
+    const float total = cluster_norm<P>(tab, cluster, sums);
+    if (cluster.block_rank() == 0 && threadIdx.x == 0) *norm = total;
+}
+
+// With each tensor's norm: a warp adds its tile's sum to its own row.
+template <int P>
+__global__ void __launch_bounds__(kSmallThreads)
+    norm_small_each_kernel(const __grid_constant__ SpanTable<kSmallSpans> tab, float* __restrict__ norm,
+                           float* __restrict__ norms) {
+    __shared__ ClusterSums sums;
+    __shared__ double rows[kSmallThreads / 32][kSmallSpans];
+    cg::cluster_group cluster = cg::this_cluster();
+    const Worker w = worker_of(cluster);
+    double* row = rows[threadIdx.x >> 5];
+    row[w.lane] = 0.0;
+    __syncwarp();
+    for_tiles(tab, w.id, w.count, [&](int t, int32_t tile) {
+        double v = reduce_part<P, 32>(tab, t, part_of(tab, t, tile, tile + 1), w.lane);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v = join<P>(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if (w.lane == 0) row[t] = join<P>(row[t], v);
+    });
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        double each = 0.0;
+        for (int r = 0; r < int(blockDim.x >> 5); ++r) each = join<P>(each, rows[r][threadIdx.x]);
+        sums.each[threadIdx.x] = each;
     }
-    cluster.sync();  // the others' sums stay until they are read
+    cluster.sync();
+    if (cluster.block_rank() == 0 && threadIdx.x < 32) {
+        double v = cluster_join<P>(cluster, &sums.each[threadIdx.x]);
+        if (int(threadIdx.x) < tab.count) norms[threadIdx.x] = root<P>(v);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v = join<P>(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if (threadIdx.x == 0) *norm = root<P>(v);
+    }
+    cluster.sync();
 }
 
 template <int P>
@@ -478,26 +524,18 @@ __global__ void __launch_bounds__(kSmallThreads)
     clip_small_kernel(const __grid_constant__ SpanTable<kSmallSpans> tab, float max_norm, float* __restrict__ norm) {
     __shared__ ClusterSums sums;
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = int(cluster.block_rank()), ranks = int(cluster.num_blocks());
-    run_sums<P, false>(tab, rank, ranks, sums);
-    cluster.sync();
-    const float total = root<P>(cluster_join<P>(cluster, &sums.whole));
-    cluster.sync();
-    if (rank == 0 && threadIdx.x == 0) *norm = total;
+    const float total = cluster_norm<P>(tab, cluster, sums);
+    if (cluster.block_rank() == 0 && threadIdx.x == 0) *norm = total;
     const float c = clip_coefficient(total, max_norm);
     if (c == 1.f) return;
-    const int32_t tiles = tab.first[tab.count], end = run_start(tiles, ranks, rank + 1);
-    int32_t tile = run_start(tiles, ranks, rank);
-    for (int t = owner_of(tab, tile); tile < end; ++t) {
-        const int32_t stop = min(end, tab.first[t + 1]);
-        if (stop <= tile) continue;
-        scale_part<kSmallThreads>(tab, t, part_of(tab, t, tile, stop), c);
-        tile = stop;
-    }
+    // the tiles that this warp has read, and no other
+    const Worker w = worker_of(cluster);
+    for_tiles(tab, w.id, w.count, [&](int t, int32_t tile) {
+        scale_part<32>(tab, t, part_of(tab, t, tile, tile + 1), c, w.lane);
+    });
 }
 
 // ----------------------------------------------------------------- AdamW --
-constexpr int kAdamTile = 4096;  // elements
 constexpr int kAdamLine = 64;     // elements: whole lines for every type
 constexpr int kAdamResident = 4;  // blocks an SM
 constexpr int kAdamGroups = 32;
@@ -529,6 +567,7 @@ struct AdamTable {
     AdamEntry entry[N];
     int32_t first[N + 1];
     int32_t count;
+    int32_t tile;  // elements
     AdamHyper hyper[kAdamGroups];
 };
 
@@ -584,11 +623,11 @@ __device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const floa
     }
 }
 
-// The update over the numbers [lo, hi) of a tensor, by the block.  kF32: all
+// The update over the numbers [lo, hi) of a tensor, by a team of T threads.  kF32: all
 // arrays are in 32 bits and there is no master, so no branch on the types
 // stands between the loads.
 template <bool kF32, int T>
-__device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const AdamScale& h) {
+__device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const AdamScale& h, int me) {
     const int pd = kF32 ? XSG_F32 : e.param_dtype, gd = kF32 ? XSG_F32 : e.grad_dtype;
     float* master = kF32 ? nullptr : e.master;
     // rows: of the part's first element by one 64-bit division, of the others
@@ -608,14 +647,14 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
         store_as(e.param, pd, i, w);
     };
     if (!e.vec) {
-        for (int64_t i = part.lo + threadIdx.x; i < part.hi; i += T) one(i);
+        for (int64_t i = part.lo + me; i < part.hi; i += T) one(i);
         return;
     }
     constexpr int L = kAdamLine;
     const int64_t first = (part.lo + L - 1) / L * (L / 4), last = part.hi / 4;
     const int n = int(max(last - first, int64_t(0)));
     const uint32_t skew = rem0 + uint32_t(4 * first - part.lo);  // of vector 0 from the row's start
-    for (int at = threadIdx.x; at < n; at += T) {
+    for (int at = me; at < n; at += T) {
         uint32_t keep = 15u;
         if (e.rows) {
             const uint32_t x = skew + 4u * uint32_t(at), r = x / rs, rem = x - r * rs;
@@ -654,16 +693,18 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
         }
     }
     const int64_t head = min(first * 4, part.hi), tail = max(last * 4, head);
-    const int64_t odd = threadIdx.x < L ? part.lo + threadIdx.x : tail + threadIdx.x - L;
-    if (threadIdx.x < 2 * L && odd < (threadIdx.x < L ? head : part.hi)) one(odd);
+    for (int j = me; j < 2 * L; j += T) {
+        const int64_t odd = j < L ? part.lo + j : tail + j - L;
+        if (odd < (j < L ? head : part.hi)) one(odd);
+    }
 }
 
-// The tiles of block b of `blocks`, in turn (a part of a masked tensor may
+// The tiles of team b of `teams`, in turn (a part of a masked tensor may
 // have little to do) and from the last to the first, as in clipping.
 template <bool kF32, int T, typename Table>
-__device__ __forceinline__ void adam_tiles(const Table& tab, int32_t b, int32_t blocks, float steps, AdamScale& h) {
+__device__ __forceinline__ void adam_tiles(const Table& tab, int32_t b, int32_t teams, int me, float steps, AdamScale& h) {
     int t = -1;
-    for (int32_t tile = tab.first[tab.count] - 1 - b; tile >= 0; tile -= blocks) {
+    for (int32_t tile = tab.first[tab.count] - 1 - b; tile >= 0; tile -= teams) {
         if (t < 0 || tile < tab.first[t]) {
             if (t < 0) t = owner_of(tab, tile);
             while (tile < tab.first[t]) --t;
@@ -675,8 +716,8 @@ __device__ __forceinline__ void adam_tiles(const Table& tab, int32_t b, int32_t 
             h.root_scale = rsqrtf(-expm1f(steps * y.log_beta2));
         }
         const AdamEntry& e = tab.entry[t];
-        const int64_t at = int64_t(tile - tab.first[t]) * kAdamTile;
-        adam_part<kF32, T>(e, {max(int64_t(e.lead), at), min(e.end, at + kAdamTile)}, h);
+        const int64_t at = int64_t(tile - tab.first[t]) * tab.tile;
+        adam_part<kF32, T>(e, {max(int64_t(e.lead), at), min(e.end, at + tab.tile)}, h, me);
     }
 }
 
@@ -705,7 +746,7 @@ __global__ void __launch_bounds__(kOptThreads, kAdamResident)
         if (call.skip_nonfinite && !isfinite(total)) return;  // every block alike: nothing changes
         if (call.clip) h.c = clip_coefficient(total, call.max_norm);
     }
-    adam_tiles<kF32, kOptThreads>(tab, blockIdx.x, gridDim.x, float(call.step[0] + 1), h);
+    adam_tiles<kF32, kOptThreads>(tab, blockIdx.x, gridDim.x, threadIdx.x, float(call.step[0] + 1), h);
     if (call.advance) count_update(call.step);
 }
 
@@ -716,18 +757,16 @@ __global__ void __launch_bounds__(kSmallThreads)
                        const __grid_constant__ AdamTable<kSmallSpans> tab, const __grid_constant__ AdamCall call) {
     __shared__ ClusterSums sums;
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = int(cluster.block_rank()), ranks = int(cluster.num_blocks());
-    run_sums<2, false>(grads, rank, ranks, sums);
-    cluster.sync();
-    const float total = root<2>(cluster_join<2>(cluster, &sums.whole));
     const float steps = float(call.step[0] + 1);
-    cluster.sync();
-    if (rank == 0 && threadIdx.x == 0 && call.norm) *call.norm = total;
+    const float total = cluster_norm<2>(grads, cluster, sums);
+    const bool first = cluster.block_rank() == 0 && threadIdx.x == 0;
+    if (first && call.norm) *call.norm = total;
     if (call.skip_nonfinite && !isfinite(total)) return;
     AdamScale h;
     h.c = call.clip ? clip_coefficient(total, call.max_norm) : 1.f;
-    adam_tiles<kF32, kSmallThreads>(tab, rank, ranks, steps, h);
-    if (rank == 0 && threadIdx.x == 0) call.step[0] += 1;  // all blocks have read it
+    const Worker w = worker_of(cluster);
+    adam_tiles<kF32, 32>(tab, w.id, w.count, w.lane, steps, h);
+    if (first) call.step[0] += 1;  // all have read it before the norm's barriers
 }
 
 // ------------------------------------------------------------------ host --
@@ -738,6 +777,16 @@ static_assert(sizeof(SpanTable<kSpans>) <= 32000 && sizeof(AdamTable<kAdamSpans>
 // One launch of a cluster against two of the whole GPU.
 constexpr int64_t kSmallNormBytes = 1 << 20;
 constexpr int64_t kSmallAdamElems = 1 << 16;
+constexpr int32_t kSmallAdamTile = 256;  // elements, a warp's: two vectors a lane
+
+bool small_norm(int64_t n_spans, int64_t bytes) { return n_spans <= kSmallSpans && bytes <= kSmallNormBytes; }
+bool small_adamw(int64_t n_spans, int64_t elems) { return n_spans <= kSmallSpans && elems <= kSmallAdamElems; }
+
+// The smallest tile that leaves a block one, up to `most`.
+int32_t tile_for(int64_t size, int32_t least, int32_t most, int64_t blocks) {
+    while (least < most && size > least * blocks) least *= 2;
+    return least;
+}
 
 template <typename T>
 struct Same {
@@ -795,31 +844,34 @@ struct SpanLaunch {
     int64_t first_span = 0, sums_at = 0, slots_at = 0, bytes = 0;
 
     void add(const void* data, int64_t n, int dtype) {
-        const int t = tab.count;
-        const int64_t per = kTileBytes / elem_size(dtype);
+        const int t = tab.count++;
         const auto at = reinterpret_cast<uintptr_t>(data);
-        const int64_t lead = int64_t(at % kLine) / elem_size(dtype);
         tab.base[t] = reinterpret_cast<void*>(at - at % kLine);
-        tab.lead[t] = uint8_t(lead);
-        tab.end[t] = lead + n;
+        tab.lead[t] = uint8_t(at % kLine / elem_size(dtype));
+        tab.end[t] = tab.lead[t] + n;
         tab.dtype[t] = uint8_t(dtype);
         bytes += n * elem_size(dtype);
-        tab.first[t + 1] = int32_t(tab.first[t] + (n ? (lead + n + per - 1) / per : 0));
-        tab.count = t + 1;
     }
-    // Blocks and slots, when all tensors are in.
+    // The tiles, when all tensors are in.
+    int32_t cut(int32_t tile_bytes) {
+        tab.tile_bytes = tile_bytes;
+        int64_t tiles = 0;
+        for (int t = 0; t < tab.count; ++t) {
+            const int64_t per = tile_bytes / elem_size(tab.dtype[t]);
+            tab.first[t] = int32_t(tiles);
+            tiles += tab.end[t] > tab.lead[t] ? (tab.end[t] + per - 1) / per : 0;
+        }
+        tab.first[tab.count] = int32_t(tiles);
+        return int32_t(tiles);
+    }
     void close(int64_t& sums, int64_t& slots) {
-        const int32_t tiles = tab.first[tab.count];
-        blocks = std::max(1, std::min(tiles, kOptBlocks));
+        blocks = std::max(1, std::min(cut(tile_for(bytes, 4096, 16384, kOptBlocks)), kOptBlocks));
         sums_at = sums;
         sums += blocks;
         slots_at = slots;
         slots += blocks + tab.count;
     }
-    SpanLaunch() {
-        tab.count = 0;
-        tab.first[0] = 0;
-    }
+    SpanLaunch() { tab.count = 0; }
 };
 
 size_t sums_count(int64_t n_spans) { return size_t((n_spans + kSpans - 1) / kSpans) * kOptBlocks; }
@@ -842,13 +894,7 @@ struct SpanPlan {
         for (auto& L : launches) L.close(sums, slots);
     }
 
-    bool small(int64_t limit) const { return N == kSmallSpans && launches[0].bytes <= limit; }
-
-    unsigned cluster() const {
-        unsigned c = 1;
-        while (c < kSmallBlocks && int32_t(c) < launches[0].blocks) c *= 2;
-        return c;
-    }
+    int64_t bytes() const { return launches[0].bytes; }
 
     template <int P>
     void partials(double* sums_at, double* slots_at, cudaStream_t st) const {
@@ -863,18 +909,33 @@ struct SpanPlan {
     }
 };
 
+// The cluster's form of a launch: its table cut into warps' tiles, and as many
+// threads as there are tiles, up to kSmallBlocks blocks.
+struct SmallLaunch {
+    SpanTable<kSmallSpans> tab;
+    unsigned cluster = 1, threads = 32;
+
+    explicit SmallLaunch(const SpanPlan<kSmallSpans>& plan) {
+        SpanLaunch<kSmallSpans> L = plan.launches[0];
+        const int32_t tiles = L.cut(kSmallTile);
+        while (threads < kSmallThreads && int32_t(threads) < 32 * tiles) threads *= 2;
+        while (cluster < kSmallBlocks && int32_t(cluster) * (kSmallThreads / 32) < tiles) cluster *= 2;
+        tab = L.tab;
+    }
+};
+
 template <int P, int N>
 int norm_all(const SpanPlan<N>& plan, float* norm, float* norms, Arena arena, int64_t n, cudaStream_t st) {
     if constexpr (N == kSmallSpans) {
-        if (plan.small(kSmallNormBytes)) {
-            launch_table(norm_small_kernel<P>, plan.cluster(), kSmallThreads, plan.cluster(), false, st,
-                         plan.launches[0].tab, norm, norms);
+        if (small_norm(n, plan.bytes())) {
+            const SmallLaunch s(plan);
+            if (norms) launch_table(norm_small_each_kernel<P>, s.cluster, s.threads, s.cluster, false, st, s.tab, norm, norms);
+            else launch_table(norm_small_kernel<P>, s.cluster, s.threads, s.cluster, false, st, s.tab, norm);
             return XSG_OK;
         }
     }
     double* sums = arena.take<double>(sums_count(n));
     double* slots = norms ? arena.take<double>(slots_count(n)) : nullptr;
-    if (!sums || (norms && !slots)) return set_error(XSG_ERR_WORKSPACE, "grad_norm: workspace too small");
     plan.template partials<P>(sums, slots, st);
     for (size_t l = 0; l < plan.launches.size(); ++l) {
         const SpanLaunch<N>& L = plan.launches[l];
@@ -891,14 +952,13 @@ int norm_all(const SpanPlan<N>& plan, float* norm, float* norms, Arena arena, in
 template <int P, int N>
 int clip_all(const SpanPlan<N>& plan, float max_norm, float* norm, Arena arena, int64_t n, cudaStream_t st) {
     if constexpr (N == kSmallSpans) {
-        if (plan.small(kSmallNormBytes)) {
-            launch_table(clip_small_kernel<P>, plan.cluster(), kSmallThreads, plan.cluster(), false, st,
-                         plan.launches[0].tab, max_norm, norm);
+        if (small_norm(n, plan.bytes())) {
+            const SmallLaunch s(plan);
+            launch_table(clip_small_kernel<P>, s.cluster, s.threads, s.cluster, false, st, s.tab, max_norm, norm);
             return XSG_OK;
         }
     }
     double* sums = arena.take<double>(sums_count(n));
-    if (!sums) return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
     plan.template partials<P>(sums, nullptr, st);
     for (size_t l = plan.launches.size(); l-- > 0;)
         launch_table(clip_scale_kernel<P, N>, plan.launches[l].blocks, kOptThreads, 1, l + 1 == plan.launches.size(),
@@ -928,7 +988,8 @@ int grad_norm(const xsg_span* spans, int64_t n, int norm_type, float* norm, floa
               cudaStream_t st) {
     if (int rc = check_spans(spans, n, "grad_norm")) return rc;
     XSG_REQUIRE(norm, "grad_norm: null output");
-    if (arena.cap < xsg_grad_norm_workspace_size(n)) return set_error(XSG_ERR_WORKSPACE, "grad_norm: workspace too small");
+    if (arena.cap < xsg_grad_norm_workspace_bytes(spans, n))
+        return set_error(XSG_ERR_WORKSPACE, "grad_norm: workspace too small");
     const auto get = [&](int64_t i, auto& L) { L.add(spans[i].data, spans[i].n, spans[i].dtype); };
     const int rc = with_plan(n, get, [&](const auto& plan) {
         return with_norm_type(norm_type, "grad_norm",
@@ -942,7 +1003,8 @@ int clip_grads(const xsg_span* spans, int64_t n, int norm_type, float max_norm, 
     if (int rc = check_spans(spans, n, "clip_grads")) return rc;
     XSG_REQUIRE(norm, "clip_grads: null output");
     XSG_REQUIRE(max_norm >= 0.f && std::isfinite(max_norm), "clip_grads: max_norm must be finite and not negative");
-    if (arena.cap < xsg_grad_norm_workspace_size(n)) return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
+    if (arena.cap < xsg_grad_norm_workspace_bytes(spans, n))
+        return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
     const auto get = [&](int64_t i, auto& L) { L.add(spans[i].data, spans[i].n, spans[i].dtype); };
     const int rc = with_plan(n, get, [&](const auto& plan) {
         return with_norm_type(norm_type, "clip_grads",
@@ -1001,9 +1063,10 @@ AdamHyper hyper_of(const xsg_adamw_span& s) {
 // Fills a table with tensors from `i` on, as many as it holds (tensors and
 // different groups of options); returns the first that is not in.
 template <int N>
-int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int64_t n, bool& f32) {
+int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int64_t n, int32_t tile, bool& f32) {
     int groups = 0, t = 0, g = 0;
     int64_t tiles = 0;
+    tab.tile = tile;
     f32 = true;
     for (; t < N && i < n; ++t, ++i) {
         const xsg_adamw_span& s = spans[i];
@@ -1037,7 +1100,7 @@ int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int
         e.grad_dtype = uint8_t(s.grad_dtype);
         f32 = f32 && s.param_dtype == XSG_F32 && s.grad_dtype == XSG_F32 && !s.master;
         tab.first[t] = int32_t(tiles);
-        tiles += s.n ? (e.lead + s.n + kAdamTile - 1) / kAdamTile : 0;
+        tiles += s.n ? (e.lead + s.n + tile - 1) / tile : 0;
     }
     tab.first[t] = int32_t(tiles);
     tab.count = t;
@@ -1045,12 +1108,13 @@ int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int
 }
 
 template <int N>
-void adamw_all(const xsg_adamw_span* spans, int64_t n, AdamCall call, float* norm, cudaStream_t st) {
+void adamw_all(const xsg_adamw_span* spans, int64_t n, int64_t elems, AdamCall call, float* norm, cudaStream_t st) {
     AdamTable<N> tab;
+    const int32_t tile = tile_for(elems, 1024, 4096, 148 * kAdamResident);
     bool pdl = call.sums != nullptr;  // the first launch follows the norm's first pass directly
     for (int64_t i = 0; i < n;) {
         bool f32;
-        i = fill_adam(tab, spans, i, n, f32);
+        i = fill_adam(tab, spans, i, n, tile, f32);
         call.advance = i >= n;
         call.norm = i >= n ? norm : nullptr;
         const int blocks = std::max(1, std::min(tab.first[tab.count], 148 * kAdamResident));
@@ -1069,24 +1133,24 @@ int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float ma
     call.clip = max_norm >= 0.f;
     call.skip_nonfinite = skip_nonfinite;
     call.max_norm = max_norm;
+    int64_t elems = 0;
+    for (int64_t i = 0; i < n; ++i) elems += spans[i].n;
     int rc = XSG_OK;
     bool done = false;
     if (call.clip || skip_nonfinite || norm) {
-        if (arena.cap < xsg_grad_norm_workspace_size(n))
+        if (arena.cap < xsg_adamw_workspace_bytes(spans, n))
             return set_error(XSG_ERR_WORKSPACE, "adamw_update: workspace too small");
         const auto get = [&](int64_t i, auto& L) { L.add(spans[i].grad, spans[i].n, spans[i].grad_dtype); };
         rc = with_plan(n, get, [&](const auto& plan) {
-            const auto& first = plan.launches[0];
-            int64_t elems = 0;
-            for (int64_t i = 0; i < n; ++i) elems += spans[i].n;
-            if constexpr (std::is_same_v<decltype(first.tab), SpanTable<kSmallSpans>>) {
-                if (elems <= kSmallAdamElems) {
+            if constexpr (std::is_same_v<std::decay_t<decltype(plan)>, SpanPlan<kSmallSpans>>) {
+                if (small_adamw(n, elems)) {
+                    const SmallLaunch s(plan);
                     AdamTable<kSmallSpans> tab;
                     bool f32;
-                    fill_adam(tab, spans, 0, n, f32);
+                    fill_adam(tab, spans, 0, n, kSmallAdamTile, f32);
                     call.norm = norm;
-                    launch_table(f32 ? adamw_small_kernel<true> : adamw_small_kernel<false>, plan.cluster(),
-                                 kSmallThreads, plan.cluster(), false, st, first.tab, tab, call);
+                    launch_table(f32 ? adamw_small_kernel<true> : adamw_small_kernel<false>, s.cluster, s.threads,
+                                 s.cluster, false, st, s.tab, tab, call);
                     done = true;
                     return int(XSG_OK);
                 }
@@ -1100,8 +1164,8 @@ int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float ma
     }
     if (rc) return rc;
     if (!done) {
-        if (n <= kSmallSpans) adamw_all<kSmallSpans>(spans, n, call, norm, st);
-        else adamw_all<kAdamSpans>(spans, n, call, norm, st);
+        if (n <= kSmallSpans) adamw_all<kSmallSpans>(spans, n, elems, call, norm, st);
+        else adamw_all<kAdamSpans>(spans, n, elems, call, norm, st);
     }
     return check_launch("adamw_update");
 }
@@ -1126,6 +1190,20 @@ using namespace xsg;
 extern "C" size_t xsg_grad_norm_workspace_size(int64_t n_spans) {
     if (n_spans <= 0) return 0;
     return Arena::round(sums_count(n_spans) * sizeof(double)) + Arena::round(slots_count(n_spans) * sizeof(double));
+}
+
+extern "C" size_t xsg_grad_norm_workspace_bytes(const xsg_span* spans_host, int64_t n_spans) {
+    if (n_spans <= 0 || !spans_host) return 0;
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < n_spans && n_spans <= kSmallSpans; ++i) bytes += spans_host[i].n * elem_size(spans_host[i].dtype);
+    return small_norm(n_spans, bytes) ? 0 : xsg_grad_norm_workspace_size(n_spans);
+}
+
+extern "C" size_t xsg_adamw_workspace_bytes(const xsg_adamw_span* spans_host, int64_t n_spans) {
+    if (n_spans <= 0 || !spans_host) return 0;
+    int64_t elems = 0;
+    for (int64_t i = 0; i < n_spans && n_spans <= kSmallSpans; ++i) elems += spans_host[i].n;
+    return small_adamw(n_spans, elems) ? 0 : xsg_grad_norm_workspace_size(n_spans);
 }
 
 extern "C" int xsg_grad_norm(const xsg_span* spans_host, int64_t n_spans, int norm_type, float* norm, float* norms,

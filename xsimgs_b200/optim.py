@@ -35,7 +35,7 @@ def gradient_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0, per_ten
     gradients neither overflow nor vanish on the way; NaN and infinite
     elements show in the result.  A tensor with gaps or expanded dimensions is
     copied first."""
-    return _C.gradient_norm(grads if isinstance(grads, list) else list(grads), norm_type, per_tensor)
+    return _C.gradient_norm(grads, norm_type, per_tensor)
 
 
 def clip_gradients_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
@@ -43,17 +43,13 @@ def clip_gradients_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: f
     returns the norm that they had.  An infinite norm gives the factor 0, a
     NaN makes every gradient NaN.  The tensors must be dense and may not share
     memory."""
-    return _C.clip_gradients_(grads if isinstance(grads, list) else list(grads), max_norm, norm_type)
+    return _C.clip_gradients_(grads, max_norm, norm_type)
 
 
 def adamw_step_counter(device, updates: int = 0) -> torch.Tensor:
     """The `step` of `adamw_update_`: the number of updates taken, which the
     call advances on the device, and a word that is zero between calls."""
     return torch.tensor([updates, 0], dtype=torch.int64, device=device)
-
-
-def _values(v) -> list:
-    return [float(x) for x in v] if isinstance(v, (list, tuple)) else [float(v)]
 
 
 def adamw_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
@@ -81,11 +77,8 @@ def adamw_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     masters have their parameter's sizes and order of dimensions.  A gradient
     in another order is copied first.  Under graph capture the learning rate
     is the one at capture."""
-    as_list = lambda v: v if isinstance(v, list) else list(v)  # noqa: E731
-    masks = [] if row_mask is None else [row_mask] if isinstance(row_mask, torch.Tensor) else list(row_mask)
-    return _C.adamw_update_(as_list(params), as_list(grads), as_list(exp_avgs), as_list(exp_avg_sqs), step,
-                            _values(lr), _values(betas[0]), _values(betas[1]), _values(eps), _values(weight_decay),
-                            max_norm, skip_nonfinite, [] if masters is None else as_list(masters), masks)
+    return _C.adamw_update_(params, grads, exp_avgs, exp_avg_sqs, step, lr, betas[0], betas[1], eps, weight_decay,
+                            max_norm, skip_nonfinite, masters, row_mask)
 
 
 class AdamW(torch.optim.Optimizer):
