@@ -551,6 +551,7 @@ typedef struct xsg_span {
  * (0 where one launch does without). */
 size_t xsg_grad_norm_workspace_size(int64_t n_spans);
 size_t xsg_grad_norm_workspace_bytes(const xsg_span* spans_host, int64_t n_spans);
+size_t xsg_clip_grads_workspace_bytes(const xsg_span* spans_host, int64_t n_spans);
 /* norm [1] = the norm of all elements of all tensors; norms [n_spans] (may be
  * NULL) = each tensor's.  NaN and infinite elements give a NaN or infinite
  * norm. */

@@ -922,7 +922,7 @@ std::tuple<Tensor, Tensor, Tensor> interpolate_smpl_bwd(const Tensor& poses, con
 // spends its host time here.
 struct TensorList {
     py::object seq;  // a list or a tuple
-    std::vector<const Tensor*> at;
+    c10::SmallVector<const Tensor*, 16> at;
 
     TensorList(const py::object& o, const char* name, bool optional = false) {
         seq = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), name));
@@ -946,7 +946,7 @@ struct TensorList {
 
 // One number for all tensors, or one for each.
 struct Numbers {
-    std::vector<double> v;
+    c10::SmallVector<double, 16> v;
 
     Numbers(const py::object& o, size_t n, const char* name) {
         if (PyList_Check(o.ptr()) || PyTuple_Check(o.ptr())) {
@@ -1004,13 +1004,15 @@ struct Extent {
     bool written;
 };
 
-void add_extent(std::vector<Extent>& e, const Tensor& t, bool written) {
+using Extents = c10::SmallVector<Extent, 72>;
+
+void add_extent(Extents& e, const Tensor& t, bool written) {
     if (t.numel() == 0) return;
     const auto p = reinterpret_cast<uintptr_t>(t.data_ptr());
     e.push_back({p, p + size_t(t.numel()) * t.element_size(), written});
 }
 
-void check_apart(std::vector<Extent>& e, const char* what) {
+void check_apart(Extents& e, const char* what) {
     std::sort(e.begin(), e.end(), [](const Extent& a, const Extent& b) { return a.begin < b.begin; });
     uintptr_t any = 0, written = 0;
     for (const Extent& x : e) {
@@ -1028,15 +1030,25 @@ int norm_code(double p) {
     return XSG_NORM_INF;
 }
 
-// Scratch of a norm; none where one launch does without.
-struct NormScratch {
-    Tensor t;
+// A norm and the scratch behind it in one allocation; the norm is a 0-dim
+// tensor on its first word (a second allocation costs a microsecond, a tenth
+// of a call over small tensors).
+struct NormOutput {
+    Tensor buffer, norm;
     size_t bytes;
-    NormScratch(const std::vector<xsg_span>& spans, const Tensor& like)
-        : bytes(xsg_grad_norm_workspace_bytes(spans.data(), int64_t(spans.size()))) {
-        if (bytes) t = workspace(bytes, like);
+    NormOutput(size_t scratch, const Tensor& like) : bytes(scratch) {
+        const auto f32 = like.options().dtype(at::kFloat).requires_grad(false);
+        if (!bytes) {
+            norm = at::empty({}, f32);
+            return;
+        }
+        buffer = at::empty({int64_t(kWords + (bytes + 3) / 4)}, f32);
+        norm = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buffer.storage()),
+                                                        buffer.key_set(), buffer.dtype());
+        norm.unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef{}, c10::IntArrayRef{});
     }
-    void* data() const { return bytes ? t.data_ptr() : nullptr; }
+    void* scratch() const { return bytes ? fptr_mut(buffer) + kWords : nullptr; }
+    static constexpr int kWords = 64;  // keeps the scratch on a 256-byte boundary
 };
 
 py::object gradient_norm(const py::object& grads_seq, double norm_type, bool per_tensor) {
@@ -1044,7 +1056,7 @@ py::object gradient_norm(const py::object& grads_seq, double norm_type, bool per
     TORCH_CHECK(!grads.empty(), "gradient_norm: at least one tensor is needed");
     const int p = norm_code(norm_type);
     std::vector<Tensor> copies;  // of tensors with gaps or expanded dimensions
-    std::vector<xsg_span> spans(grads.size());
+    c10::SmallVector<xsg_span, 16> spans(grads.size());
     require_cuda(grads[0], "grads");
     c10::cuda::CUDAGuard g(grads[0].device());
     for (size_t i = 0; i < grads.size(); ++i) {
@@ -1056,13 +1068,12 @@ py::object gradient_norm(const py::object& grads_seq, double norm_type, bool per
         spans[i] = {t.data_ptr(), t.numel(), dtype};
     }
     const auto f32 = grads[0].options().dtype(at::kFloat).requires_grad(false);
-    Tensor norm = at::empty({}, f32);
+    const NormOutput out(xsg_grad_norm_workspace_bytes(spans.data(), int64_t(spans.size())), grads[0]);
     Tensor norms = per_tensor ? at::empty({int64_t(grads.size())}, f32) : Tensor();
-    const NormScratch ws(spans, norm);
-    check(xsg_grad_norm(spans.data(), int64_t(spans.size()), p, fptr_mut(norm), per_tensor ? fptr_mut(norms) : nullptr,
-                        ws.data(), ws.bytes, stream()));
-    if (per_tensor) return py::make_tuple(norm, norms);
-    return py::cast(norm);
+    check(xsg_grad_norm(spans.data(), int64_t(spans.size()), p, fptr_mut(out.norm),
+                        per_tensor ? fptr_mut(norms) : nullptr, out.scratch(), out.bytes, stream()));
+    if (per_tensor) return py::make_tuple(out.norm, norms);
+    return py::cast(out.norm);
 }
 
 Tensor clip_gradients(const py::object& grads_seq, double max_norm, double norm_type) {
@@ -1071,8 +1082,8 @@ Tensor clip_gradients(const py::object& grads_seq, double max_norm, double norm_
     const int p = norm_code(norm_type);
     TORCH_CHECK(std::isfinite(max_norm) && max_norm >= 0.0 && max_norm <= std::numeric_limits<float>::max(),
                 "clip_gradients_: max_norm must be finite and not negative, got ", max_norm);
-    std::vector<xsg_span> spans(grads.size());
-    std::vector<Extent> extents;
+    c10::SmallVector<xsg_span, 16> spans(grads.size());
+    Extents extents;
     require_cuda(grads[0], "grads");
     for (size_t i = 0; i < grads.size(); ++i) {
         check_written(grads[i], "grads", grads[0]);
@@ -1081,12 +1092,11 @@ Tensor clip_gradients(const py::object& grads_seq, double max_norm, double norm_
     }
     check_apart(extents, "clip_gradients_");
     c10::cuda::CUDAGuard g(grads[0].device());
-    Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
-    const NormScratch ws(spans, norm);
+    const NormOutput out(xsg_clip_grads_workspace_bytes(spans.data(), int64_t(spans.size())), grads[0]);
     for (size_t i = 0; i < grads.size(); ++i) torch::autograd::impl::bump_version(grads[i]);
-    check(xsg_clip_grads(spans.data(), int64_t(spans.size()), p, float(max_norm), fptr_mut(norm), ws.data(), ws.bytes,
-                         stream()));
-    return norm;
+    check(xsg_clip_grads(spans.data(), int64_t(spans.size()), p, float(max_norm), fptr_mut(out.norm), out.scratch(),
+                         out.bytes, stream()));
+    return out.norm;
 }
 
 std::optional<Tensor> adamw_update(const py::object& params_seq, const py::object& grads_seq,
@@ -1117,9 +1127,9 @@ std::optional<Tensor> adamw_update(const py::object& params_seq, const py::objec
     TORCH_CHECK(step.scalar_type() == at::kLong && step.numel() == 2 && step.is_contiguous(),
                 "adamw_update_: step must be a contiguous int64 tensor of two words (adamw_step_counter)");
     c10::cuda::CUDAGuard g(params[0].device());
-    std::vector<xsg_adamw_span> spans(n);
+    c10::SmallVector<xsg_adamw_span, 16> spans(n);
     std::vector<Tensor> copies;  // of gradients whose order of dimensions is not their parameter's
-    std::vector<Extent> extents;
+    Extents extents;
     extents.reserve(5 * n + 1);
     add_extent(extents, step, true);
     for (size_t i = 0; i < n; ++i) {
@@ -1177,13 +1187,8 @@ std::optional<Tensor> adamw_update(const py::object& params_seq, const py::objec
     }
     check_apart(extents, "adamw_update_");
     const bool normed = max_norm.has_value() || skip_nonfinite;
-    Tensor norm, ws;
-    size_t bytes = 0;
-    if (normed) {
-        norm = at::empty({}, params[0].options().dtype(at::kFloat).requires_grad(false));
-        bytes = xsg_adamw_workspace_bytes(spans.data(), int64_t(n));
-        if (bytes) ws = workspace(bytes, norm);
-    }
+    std::optional<NormOutput> out;
+    if (normed) out.emplace(xsg_adamw_workspace_bytes(spans.data(), int64_t(n)), params[0]);
     for (size_t i = 0; i < n; ++i) {
         torch::autograd::impl::bump_version(params[i]);
         torch::autograd::impl::bump_version(exp_avgs[i]);
@@ -1191,9 +1196,9 @@ std::optional<Tensor> adamw_update(const py::object& params_seq, const py::objec
         if (spans[i].master) torch::autograd::impl::bump_version((*masters)[i]);
     }
     check(xsg_adamw_update(spans.data(), int64_t(n), step.data_ptr<int64_t>(), max_norm ? float(*max_norm) : -1.f,
-                           skip_nonfinite, normed ? fptr_mut(norm) : nullptr, bytes ? ws.data_ptr() : nullptr, bytes,
-                           stream()));
-    return normed ? std::optional<Tensor>(norm) : std::nullopt;
+                           skip_nonfinite, out ? fptr_mut(out->norm) : nullptr, out ? out->scratch() : nullptr,
+                           out ? out->bytes : 0, stream()));
+    return out ? std::optional<Tensor>(out->norm) : std::nullopt;
 }
 
 }  // namespace

@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kOptThreads, kOptResident)
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallBlocks = 8;
 constexpr int kSmallSpans = 32;
-constexpr int kSmallTile = 2048;  // bytes: four vectors a lane
+constexpr int kSmallTile = 4096;  // bytes: eight vectors a lane
 
 // A block's sums, where the others of the cluster read them.
 struct ClusterSums {
@@ -776,10 +776,12 @@ static_assert(sizeof(SpanTable<kSpans>) <= 32000 && sizeof(AdamTable<kAdamSpans>
               "kernel parameters hold 32764 bytes");
 // One launch of a cluster against two of the whole GPU.
 constexpr int64_t kSmallNormBytes = 1 << 20;
-constexpr int64_t kSmallAdamElems = 1 << 16;
+constexpr int64_t kSmallClipBytes = 1 << 18;
+constexpr int64_t kSmallAdamElems = 1 << 11;
 constexpr int32_t kSmallAdamTile = 256;  // elements, a warp's: two vectors a lane
 
 bool small_norm(int64_t n_spans, int64_t bytes) { return n_spans <= kSmallSpans && bytes <= kSmallNormBytes; }
+bool small_clip(int64_t n_spans, int64_t bytes) { return n_spans <= kSmallSpans && bytes <= kSmallClipBytes; }
 bool small_adamw(int64_t n_spans, int64_t elems) { return n_spans <= kSmallSpans && elems <= kSmallAdamElems; }
 
 // The smallest tile that leaves a block one, up to `most`.
@@ -952,7 +954,7 @@ int norm_all(const SpanPlan<N>& plan, float* norm, float* norms, Arena arena, in
 template <int P, int N>
 int clip_all(const SpanPlan<N>& plan, float max_norm, float* norm, Arena arena, int64_t n, cudaStream_t st) {
     if constexpr (N == kSmallSpans) {
-        if (small_norm(n, plan.bytes())) {
+        if (small_clip(n, plan.bytes())) {
             const SmallLaunch s(plan);
             launch_table(clip_small_kernel<P>, s.cluster, s.threads, s.cluster, false, st, s.tab, max_norm, norm);
             return XSG_OK;
@@ -1003,7 +1005,7 @@ int clip_grads(const xsg_span* spans, int64_t n, int norm_type, float max_norm, 
     if (int rc = check_spans(spans, n, "clip_grads")) return rc;
     XSG_REQUIRE(norm, "clip_grads: null output");
     XSG_REQUIRE(max_norm >= 0.f && std::isfinite(max_norm), "clip_grads: max_norm must be finite and not negative");
-    if (arena.cap < xsg_grad_norm_workspace_bytes(spans, n))
+    if (arena.cap < xsg_clip_grads_workspace_bytes(spans, n))
         return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
     const auto get = [&](int64_t i, auto& L) { L.add(spans[i].data, spans[i].n, spans[i].dtype); };
     const int rc = with_plan(n, get, [&](const auto& plan) {
@@ -1192,11 +1194,21 @@ extern "C" size_t xsg_grad_norm_workspace_size(int64_t n_spans) {
     return Arena::round(sums_count(n_spans) * sizeof(double)) + Arena::round(slots_count(n_spans) * sizeof(double));
 }
 
+// Bytes of at most kSmallSpans tensors (no more are asked for).
+static int64_t small_bytes(const xsg_span* spans, int64_t n) {
+    int64_t bytes = 0;
+    for (int64_t i = 0; i < n && n <= kSmallSpans; ++i) bytes += spans[i].n * elem_size(spans[i].dtype);
+    return bytes;
+}
+
 extern "C" size_t xsg_grad_norm_workspace_bytes(const xsg_span* spans_host, int64_t n_spans) {
     if (n_spans <= 0 || !spans_host) return 0;
-    int64_t bytes = 0;
-    for (int64_t i = 0; i < n_spans && n_spans <= kSmallSpans; ++i) bytes += spans_host[i].n * elem_size(spans_host[i].dtype);
-    return small_norm(n_spans, bytes) ? 0 : xsg_grad_norm_workspace_size(n_spans);
+    return small_norm(n_spans, small_bytes(spans_host, n_spans)) ? 0 : xsg_grad_norm_workspace_size(n_spans);
+}
+
+extern "C" size_t xsg_clip_grads_workspace_bytes(const xsg_span* spans_host, int64_t n_spans) {
+    if (n_spans <= 0 || !spans_host) return 0;
+    return small_clip(n_spans, small_bytes(spans_host, n_spans)) ? 0 : xsg_grad_norm_workspace_size(n_spans);
 }
 
 extern "C" size_t xsg_adamw_workspace_bytes(const xsg_adamw_span* spans_host, int64_t n_spans) {
