@@ -537,7 +537,10 @@ __global__ void __launch_bounds__(kSmallThreads)
 
 // ----------------------------------------------------------------- AdamW --
 constexpr int kAdamLine = 64;     // elements: whole lines for every type
-constexpr int kAdamResident = 4;  // blocks an SM
+// Blocks an SM.  118 M floats, clipped: 4 of them 618 us, 5 (and spills) 632;
+// 150 M bf16 over masters, fewer bytes a thread: 4 823 us, 5 760, 6 834; 1 M
+// masked rows of 59 floats, two vectors under way a thread: 3 162 us, 4 169.
+__host__ __device__ constexpr int adam_resident(bool f32, bool rows) { return rows ? 3 : f32 ? 4 : 5; }
 constexpr int kAdamGroups = 32;
 
 struct AdamHyper {
@@ -559,6 +562,7 @@ struct AdamEntry {
     const uint8_t* rows;
     int64_t end;
     int32_t row_size;
+    uint32_t row_magic;  // 2^31 / row_size, rounded up
     uint8_t lead, vec, group, param_dtype, grad_dtype;
 };
 
@@ -626,82 +630,171 @@ __device__ __forceinline__ void store4(void* p, int dtype, int64_t i, const floa
 // The update over the numbers [lo, hi) of a tensor, by a team of T threads.  kF32: all
 // arrays are in 32 bits and there is no master, so no branch on the types
 // stands between the loads.
-template <bool kF32, int T>
-__device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const AdamScale& h, int me) {
-    const int pd = kF32 ? XSG_F32 : e.param_dtype, gd = kF32 ? XSG_F32 : e.grad_dtype;
-    float* master = kF32 ? nullptr : e.master;
-    // rows: of the part's first element by one 64-bit division, of the others
-    // by a 32-bit one of their distance (part < 2^31, row_size < 2^30)
-    const int64_t origin = part.lo - e.lead;
-    const uint32_t rs = e.rows ? uint32_t(e.row_size) : 1u;
-    const int64_t row0 = e.rows ? origin / rs : 0;
-    const uint32_t rem0 = e.rows ? uint32_t(origin - row0 * rs) : 0u;
-    const auto one = [&](int64_t i) {
-        if (e.rows && !e.rows[row0 + (rem0 + uint32_t(i - part.lo)) / rs]) return;
+template <bool kF32>
+struct AdamAt {
+    const AdamEntry& e;
+    const AdamScale& h;
+
+    __device__ __forceinline__ int param_dtype() const { return kF32 ? XSG_F32 : e.param_dtype; }
+    __device__ __forceinline__ int grad_dtype() const { return kF32 ? XSG_F32 : e.grad_dtype; }
+    __device__ __forceinline__ float* master() const { return kF32 ? nullptr : e.master; }
+
+    // Element i.
+    __device__ __forceinline__ void one(int64_t i) const {
         float m = e.exp_avg[i], v = e.exp_avg_sq[i];
-        float w = master ? master[i] : load_as(e.param, pd, i);
-        adam_element(h, load_as(e.grad, gd, i), m, v, w);
+        float w = master() ? master()[i] : load_as(e.param, param_dtype(), i);
+        adam_element(h, load_as(e.grad, grad_dtype(), i), m, v, w);
         e.exp_avg[i] = m;
         e.exp_avg_sq[i] = v;
-        if (master) master[i] = w;
-        store_as(e.param, pd, i, w);
+        if (master()) master()[i] = w;
+        store_as(e.param, param_dtype(), i, w);
+    }
+    struct Four {
+        float w[4], g[4], m[4], v[4];
     };
+    // Vector i; `keep` has a bit for each of its elements that is updated.
+    __device__ __forceinline__ void load(Four& x, int64_t i) const {
+        load4(x.g, e.grad, grad_dtype(), i);
+        load4(x.m, e.exp_avg, XSG_F32, i);
+        load4(x.v, e.exp_avg_sq, XSG_F32, i);
+        if (master()) load4(x.w, master(), XSG_F32, i);
+        else load4(x.w, e.param, param_dtype(), i);
+    }
+    __device__ __forceinline__ void update(Four& x, int64_t i, uint32_t keep) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float m = x.m[j], v = x.v[j], w = x.w[j];
+            adam_element(h, x.g[j], m, v, w);
+            if (keep >> j & 1) x.m[j] = m, x.v[j] = v, x.w[j] = w;
+        }
+        store4(e.exp_avg, XSG_F32, i, x.m);
+        store4(e.exp_avg_sq, XSG_F32, i, x.v);
+        if (master()) store4(master(), XSG_F32, i, x.w);
+        if (keep == 15u || (!master() && param_dtype() == XSG_F32)) {
+            store4(e.param, param_dtype(), i, x.w);
+        } else {
+            // a row that is passed over keeps its parameter's bits, whatever its master says
+            for (int j = 0; j < 4; ++j)
+                if (keep >> j & 1) store_as(e.param, param_dtype(), 4 * i + j, x.w[j]);
+        }
+    }
+};
+
+// Rows of a part's elements: of its first by a 64-bit division, of the others
+// from their distance x to that row's start.  x is below the row's size plus
+// a tile's 8192 + 64 elements: below twice the size of rows of 16384 and more,
+// and exact by the multiplication for shorter ones (x * size < 2^31).
+struct RowsAt {
+    const uint8_t* rows;
+    uint32_t size, rem, magic;
+
+    __device__ __forceinline__ RowsAt(const AdamEntry& e, int64_t element)
+        : size(uint32_t(e.row_size)), magic(e.row_magic) {
+        const int64_t row = element / e.row_size;
+        rows = e.rows + row;
+        rem = uint32_t(element - row * e.row_size);
+    }
+    __device__ __forceinline__ uint32_t row(uint32_t x) const {
+        return size >= 16384u ? uint32_t(x >= size) : uint32_t((uint64_t(x) * magic) >> 31);
+    }
+    // Whether the element at a distance from the first is updated.
+    __device__ __forceinline__ bool keeps(uint32_t distance) const { return rows[row(rem + distance)] != 0; }
+    // The same for four elements from there on, as bits.
+    __device__ __forceinline__ uint32_t keeps4(uint32_t distance) const {
+        const uint32_t x = rem + distance, r = row(x);
+        if (size >= 3u) {  // two rows at most
+            const uint32_t left = (r + 1u) * size - x;  // of row r
+            const uint32_t a = rows[r] ? 15u : 0u;
+            if (left >= 4u) return a;
+            const uint32_t mask = (1u << left) - 1u;
+            return (a & mask) | (rows[r + 1u] ? 15u & ~mask : 0u);
+        }
+        uint32_t k = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) k |= rows[size == 1u ? x + j : (x + j) >> 1] ? 1u << j : 0u;
+        return k;
+    }
+};
+
+template <bool kF32, bool kRows, int T>
+__device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const AdamScale& h, int me) {
+    const AdamAt<kF32> at{e, h};
+    if (kRows && e.rows) {
+        const RowsAt rows(e, part.lo - e.lead);
+        if (!e.vec) {
+            for (int64_t i = part.lo + me; i < part.hi; i += T)
+                if (rows.keeps(uint32_t(i - part.lo))) at.one(i);
+            return;
+        }
+        constexpr int L = kAdamLine;
+        const int64_t first = (part.lo + L - 1) / L * (L / 4), last = part.hi / 4;
+        const int n = int(max(last - first, int64_t(0)));
+        const uint32_t skip = uint32_t(4 * first - part.lo);
+        constexpr int kPair = T == 32 ? 1 : 2;
+        constexpr int kRowsWarps = T == 32 ? kSmallThreads / 32 : T / 32;
+        // Each warp lists the vectors of a stretch that have something to
+        // update, and then goes through the list with all lanes at work.
+        constexpr int kStretch = 8 * 32;
+        __shared__ uint16_t lists[kRowsWarps][kStretch];
+        uint16_t* list = lists[threadIdx.x >> 5];
+        const int lane = int(threadIdx.x & 31);
+        for (int base = me / 32 * kStretch; base < n; base += T / 32 * kStretch) {
+            int count = 0;
+#pragma unroll
+            for (int k = 0; k < kStretch; k += 32) {
+                const int j = base + k + lane;
+                const uint32_t keep = j < n ? rows.keeps4(skip + 4u * uint32_t(j)) : 0u;
+                const uint32_t some = __ballot_sync(0xffffffffu, keep != 0u);
+                if (keep) list[count + __popc(some & ((1u << lane) - 1u))] = uint16_t((k + lane) << 4 | keep);
+                count += __popc(some);
+            }
+            __syncwarp();
+            for (int q = lane; q < count; q += kPair * 32) {
+                typename AdamAt<kF32>::Four x[kPair];
+                int64_t i[kPair];
+                uint32_t keep[kPair];
+#pragma unroll
+                for (int p = 0; p < kPair; ++p) {
+                    const uint32_t entry = q + p * 32 < count ? list[q + p * 32] : 0u;
+                    i[p] = first + base + (entry >> 4);
+                    keep[p] = entry & 15u;
+                    if (keep[p]) at.load(x[p], i[p]);
+                }
+#pragma unroll
+                for (int p = 0; p < kPair; ++p)
+                    if (keep[p]) at.update(x[p], i[p], keep[p]);
+            }
+            __syncwarp();
+        }
+        const int64_t head = min(first * 4, part.hi), tail = max(last * 4, head);
+        for (int j = me; j < 2 * L; j += T) {
+            const int64_t odd = j < L ? part.lo + j : tail + j - L;
+            if (odd < (j < L ? head : part.hi) && rows.keeps(uint32_t(odd - part.lo))) at.one(odd);
+        }
+        return;
+    }
     if (!e.vec) {
-        for (int64_t i = part.lo + me; i < part.hi; i += T) one(i);
+        for (int64_t i = part.lo + me; i < part.hi; i += T) at.one(i);
         return;
     }
     constexpr int L = kAdamLine;
     const int64_t first = (part.lo + L - 1) / L * (L / 4), last = part.hi / 4;
     const int n = int(max(last - first, int64_t(0)));
-    const uint32_t skew = rem0 + uint32_t(4 * first - part.lo);  // of vector 0 from the row's start
-    for (int at = me; at < n; at += T) {
-        uint32_t keep = 15u;
-        if (e.rows) {
-            const uint32_t x = skew + 4u * uint32_t(at), r = x / rs, rem = x - r * rs;
-            const uint8_t* row = e.rows + row0 + r;
-            keep = row[0] ? 1u : 0u;
-#pragma unroll
-            for (uint32_t j = 1; j < 4; ++j) {
-                // element j's row: at most j rows on
-                const uint32_t y = rem + j, on = (y >= rs) + (j >= 2 && y >= 2 * rs) + (j >= 3 && y >= 3 * rs);
-                keep |= row[on] ? 1u << j : 0u;
-            }
-            if (!keep) continue;
-        }
-        const int64_t i = first + at;
-        float w[4], g[4], m[4], v[4];
-        load4(g, e.grad, gd, i);
-        load4(m, e.exp_avg, XSG_F32, i);
-        load4(v, e.exp_avg_sq, XSG_F32, i);
-        if (master) load4(w, master, XSG_F32, i);
-        else load4(w, e.param, pd, i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float nm = m[j], nv = v[j], nw = w[j];
-            adam_element(h, g[j], nm, nv, nw);
-            if (keep >> j & 1) m[j] = nm, v[j] = nv, w[j] = nw;
-        }
-        store4(e.exp_avg, XSG_F32, i, m);
-        store4(e.exp_avg_sq, XSG_F32, i, v);
-        if (master) store4(master, XSG_F32, i, w);
-        if (keep == 15u || (!master && pd == XSG_F32)) {
-            store4(e.param, pd, i, w);
-        } else {
-            // a row that is passed over keeps its parameter's bits, whatever its master says
-            for (int j = 0; j < 4; ++j)
-                if (keep >> j & 1) store_as(e.param, pd, 4 * i + j, w[j]);
-        }
+    for (int j = me; j < n; j += T) {
+        typename AdamAt<kF32>::Four x;
+        at.load(x, first + j);
+        at.update(x, first + j, 15u);
     }
     const int64_t head = min(first * 4, part.hi), tail = max(last * 4, head);
     for (int j = me; j < 2 * L; j += T) {
         const int64_t odd = j < L ? part.lo + j : tail + j - L;
-        if (odd < (j < L ? head : part.hi)) one(odd);
+        if (odd < (j < L ? head : part.hi)) at.one(odd);
     }
 }
 
 // The tiles of team b of `teams`, in turn (a part of a masked tensor may
 // have little to do) and from the last to the first, as in clipping.
-template <bool kF32, int T, typename Table>
+template <bool kF32, bool kRows, int T, typename Table>
 __device__ __forceinline__ void adam_tiles(const Table& tab, int32_t b, int32_t teams, int me, float steps, AdamScale& h) {
     int t = -1;
     for (int32_t tile = tab.first[tab.count] - 1 - b; tile >= 0; tile -= teams) {
@@ -717,7 +810,7 @@ __device__ __forceinline__ void adam_tiles(const Table& tab, int32_t b, int32_t 
         }
         const AdamEntry& e = tab.entry[t];
         const int64_t at = int64_t(tile - tab.first[t]) * tab.tile;
-        adam_part<kF32, T>(e, {max(int64_t(e.lead), at), min(e.end, at + tab.tile)}, h, me);
+        adam_part<kF32, kRows, T>(e, {max(int64_t(e.lead), at), min(e.end, at + tab.tile)}, h, me);
     }
 }
 
@@ -733,8 +826,8 @@ __device__ __forceinline__ void count_update(long long* step) {
     }
 }
 
-template <int N, bool kF32>
-__global__ void __launch_bounds__(kOptThreads, kAdamResident)
+template <int N, bool kF32, bool kRows>
+__global__ void __launch_bounds__(kOptThreads, adam_resident(kF32, kRows))
     adamw_kernel(const __grid_constant__ AdamTable<N> tab, const __grid_constant__ AdamCall call) {
     __shared__ double smem[33];
     AdamScale h;
@@ -746,7 +839,7 @@ __global__ void __launch_bounds__(kOptThreads, kAdamResident)
         if (call.skip_nonfinite && !isfinite(total)) return;  // every block alike: nothing changes
         if (call.clip) h.c = clip_coefficient(total, call.max_norm);
     }
-    adam_tiles<kF32, kOptThreads>(tab, blockIdx.x, gridDim.x, threadIdx.x, float(call.step[0] + 1), h);
+    adam_tiles<kF32, kRows, kOptThreads>(tab, blockIdx.x, gridDim.x, threadIdx.x, float(call.step[0] + 1), h);
     if (call.advance) count_update(call.step);
 }
 
@@ -765,13 +858,13 @@ __global__ void __launch_bounds__(kSmallThreads)
     AdamScale h;
     h.c = call.clip ? clip_coefficient(total, call.max_norm) : 1.f;
     const Worker w = worker_of(cluster);
-    adam_tiles<kF32, 32>(tab, w.id, w.count, w.lane, steps, h);
+    adam_tiles<kF32, true, 32>(tab, w.id, w.count, w.lane, steps, h);
     if (first) call.step[0] += 1;  // all have read it before the norm's barriers
 }
 
 // ------------------------------------------------------------------ host --
 constexpr int kSpans = 1024;
-constexpr int kAdamSpans = 400;
+constexpr int kAdamSpans = 380;
 static_assert(sizeof(SpanTable<kSpans>) <= 32000 && sizeof(AdamTable<kAdamSpans>) + sizeof(AdamCall) <= 32000,
               "kernel parameters hold 32764 bytes");
 // One launch of a cluster against two of the whole GPU.
@@ -1065,11 +1158,11 @@ AdamHyper hyper_of(const xsg_adamw_span& s) {
 // Fills a table with tensors from `i` on, as many as it holds (tensors and
 // different groups of options); returns the first that is not in.
 template <int N>
-int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int64_t n, int32_t tile, bool& f32) {
+int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int64_t n, int32_t tile, bool& f32, bool& rows) {
     int groups = 0, t = 0, g = 0;
     int64_t tiles = 0;
     tab.tile = tile;
-    f32 = true;
+    f32 = true, rows = false;
     for (; t < N && i < n; ++t, ++i) {
         const xsg_adamw_span& s = spans[i];
         const auto same = [&](const xsg_adamw_span& o) {
@@ -1097,10 +1190,12 @@ int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int
         e.master = s.master ? reinterpret_cast<float*>(back(s.master, 4)) : nullptr;
         e.rows = s.row_mask;
         e.end = e.lead + s.n;
-        e.row_size = int32_t(s.row_size);
+        e.row_size = int32_t(std::max<int64_t>(s.row_size, 1));
+        e.row_magic = uint32_t(((int64_t(1) << 31) + e.row_size - 1) / e.row_size);
         e.param_dtype = uint8_t(s.param_dtype);
         e.grad_dtype = uint8_t(s.grad_dtype);
         f32 = f32 && s.param_dtype == XSG_F32 && s.grad_dtype == XSG_F32 && !s.master;
+        rows = rows || (s.row_mask && s.n);
         tab.first[t] = int32_t(tiles);
         tiles += s.n ? (e.lead + s.n + tile - 1) / tile : 0;
     }
@@ -1112,15 +1207,19 @@ int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int
 template <int N>
 void adamw_all(const xsg_adamw_span* spans, int64_t n, int64_t elems, AdamCall call, float* norm, cudaStream_t st) {
     AdamTable<N> tab;
-    const int32_t tile = tile_for(elems, 1024, 4096, 148 * kAdamResident);
+    bool masked = false;
+    for (int64_t i = 0; i < n; ++i) masked = masked || spans[i].row_mask;
+    const int32_t tile = tile_for(elems, 1024, masked ? 8192 : 4096, kOptBlocks);
     bool pdl = call.sums != nullptr;  // the first launch follows the norm's first pass directly
     for (int64_t i = 0; i < n;) {
-        bool f32;
-        i = fill_adam(tab, spans, i, n, tile, f32);
+        bool f32, rows;
+        i = fill_adam(tab, spans, i, n, tile, f32, rows);
         call.advance = i >= n;
         call.norm = i >= n ? norm : nullptr;
-        const int blocks = std::max(1, std::min(tab.first[tab.count], 148 * kAdamResident));
-        launch_table(f32 ? adamw_kernel<N, true> : adamw_kernel<N, false>, blocks, kOptThreads, 1, pdl, st, tab, call);
+        const int blocks = std::max(1, std::min(tab.first[tab.count], 148 * adam_resident(f32, rows)));
+        launch_table(f32 ? (rows ? adamw_kernel<N, true, true> : adamw_kernel<N, true, false>)
+                         : (rows ? adamw_kernel<N, false, true> : adamw_kernel<N, false, false>),
+                     blocks, kOptThreads, 1, pdl, st, tab, call);
         pdl = false;
     }
 }
@@ -1148,8 +1247,8 @@ int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float ma
                 if (small_adamw(n, elems)) {
                     const SmallLaunch s(plan);
                     AdamTable<kSmallSpans> tab;
-                    bool f32;
-                    fill_adam(tab, spans, 0, n, kSmallAdamTile, f32);
+                    bool f32, rows;
+                    fill_adam(tab, spans, 0, n, kSmallAdamTile, f32, rows);
                     call.norm = norm;
                     launch_table(f32 ? adamw_small_kernel<true> : adamw_small_kernel<false>, s.cluster, s.threads,
                                  s.cluster, false, st, s.tab, tab, call);
