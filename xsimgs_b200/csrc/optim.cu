@@ -32,8 +32,10 @@ namespace xsg {
 namespace {
 
 constexpr int kOptThreads = 256;
-constexpr int kOptResident = 4;          // blocks an SM
-constexpr int kOptBlocks = 148 * kOptResident;  // blocks a launch at most: all of them run at once
+// Blocks of a launch at most: as many as run at once.
+constexpr int kNormResident = 5;
+constexpr int kScaleResident = 4;
+constexpr int kOptBlocks = 148 * kNormResident;
 constexpr float kClipEps = 1e-6f;
 constexpr int kNormInf = 0;
 
@@ -216,6 +218,7 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part, int m
     }
     // the elements before the first and after the last of these vectors, each fewer than a line's
     const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
+    if (head == part.lo && tail == part.hi) return acc;
     for (int j = me; j < 2 * L; j += T) {
         const int64_t odd = j < L ? part.lo + j : tail + j - L;
         if (odd < (j < L ? head : part.hi)) acc = join<P>(acc, term<P>(load_as(base, D, odd)));
@@ -260,7 +263,7 @@ __device__ __forceinline__ float clip_coefficient(float norm, float max_norm) {
 // Partial sums of a launch: sums[b] of all tiles of block b, which takes them
 // in turn.
 template <int P, int N>
-__global__ void __launch_bounds__(kOptThreads, kOptResident)
+__global__ void __launch_bounds__(kOptThreads, kNormResident)
     norm_partial_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums) {
     __shared__ double smem[33];
     pdl_trigger();
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(kOptThreads, kOptResident)
 // the runs, so that no two parts share a slot, and blocks + tensors of them
 // are enough.
 template <int P, int N>
-__global__ void __launch_bounds__(kOptThreads, kOptResident)
+__global__ void __launch_bounds__(kOptThreads, kNormResident)
     norm_partial_each_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums,
                              double* __restrict__ slots) {
     __shared__ double smem[33];
@@ -376,6 +379,7 @@ __device__ __forceinline__ void scale_part(void* base, Part part, float c, int m
                 make_uint4(scaled<D>(q[k].x, c), scaled<D>(q[k].y, c), scaled<D>(q[k].z, c), scaled<D>(q[k].w, c));
     }
     const int64_t head = min(first * V, part.hi), tail = max(last * V, head);
+    if (head == part.lo && tail == part.hi) return;
     for (int j = me; j < 2 * L; j += T) {
         const int64_t odd = j < L ? part.lo + j : tail + j - L;
         if (odd < (j < L ? head : part.hi)) store_as(base, D, odd, load_as(base, D, odd) * c);
@@ -394,7 +398,7 @@ __device__ __forceinline__ void scale_part(const Table& tab, int t, Part part, f
 // taken from the last to the first, so that what the first pass read last,
 // and the L2 still holds, comes first.
 template <int P, int N>
-__global__ void __launch_bounds__(kOptThreads, kOptResident)
+__global__ void __launch_bounds__(kOptThreads, kScaleResident)
     clip_scale_kernel(const __grid_constant__ SpanTable<N> tab, const double* sums, int n_sums,
                       float max_norm, float* __restrict__ norm) {
     __shared__ double smem[33];
@@ -767,6 +771,7 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
             __syncwarp();
         }
         const int64_t head = min(first * 4, part.hi), tail = max(last * 4, head);
+        if (head == part.lo && tail == part.hi) return;
         for (int j = me; j < 2 * L; j += T) {
             const int64_t odd = j < L ? part.lo + j : tail + j - L;
             if (odd < (j < L ? head : part.hi) && rows.keeps(uint32_t(odd - part.lo))) at.one(odd);
@@ -786,6 +791,7 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
         at.update(x, first + j, 15u);
     }
     const int64_t head = min(first * 4, part.hi), tail = max(last * 4, head);
+    if (head == part.lo && tail == part.hi) return;
     for (int j = me; j < 2 * L; j += T) {
         const int64_t odd = j < L ? part.lo + j : tail + j - L;
         if (odd < (j < L ? head : part.hi)) at.one(odd);
@@ -960,7 +966,10 @@ struct SpanLaunch {
         return int32_t(tiles);
     }
     void close(int64_t& sums, int64_t& slots) {
-        blocks = std::max(1, std::min(cut(tile_for(bytes, 4096, 16384, kOptBlocks)), kOptBlocks));
+        // from 16 KB on, larger tiles only where each block has many (118 M floats: 32 KB 236 us to clip, 16 KB 238,
+        // 64 KB 240)
+        const bool many = bytes > (int64_t(32) << 10) * kOptBlocks * 8;
+        blocks = std::max(1, std::min(cut(many ? 32768 : tile_for(bytes, 4096, 16384, kOptBlocks)), kOptBlocks));
         sums_at = sums;
         sums += blocks;
         slots_at = slots;
@@ -1056,7 +1065,7 @@ int clip_all(const SpanPlan<N>& plan, float max_norm, float* norm, Arena arena, 
     double* sums = arena.take<double>(sums_count(n));
     plan.template partials<P>(sums, nullptr, st);
     for (size_t l = plan.launches.size(); l-- > 0;)
-        launch_table(clip_scale_kernel<P, N>, plan.launches[l].blocks, kOptThreads, 1, l + 1 == plan.launches.size(),
+        launch_table(clip_scale_kernel<P, N>, std::min(plan.launches[l].blocks, 148 * kScaleResident), kOptThreads, 1, l + 1 == plan.launches.size(),
                      st, plan.launches[l].tab, sums, int(plan.sums), max_norm, l == 0 ? norm : nullptr);
     return XSG_OK;
 }
@@ -1209,7 +1218,7 @@ void adamw_all(const xsg_adamw_span* spans, int64_t n, int64_t elems, AdamCall c
     AdamTable<N> tab;
     bool masked = false;
     for (int64_t i = 0; i < n; ++i) masked = masked || spans[i].row_mask;
-    const int32_t tile = tile_for(elems, 1024, masked ? 8192 : 4096, kOptBlocks);
+    const int32_t tile = tile_for(elems, 1024, masked ? 8192 : 4096, 148 * 4);
     bool pdl = call.sums != nullptr;  // the first launch follows the norm's first pass directly
     for (int64_t i = 0; i < n;) {
         bool f32, rows;
