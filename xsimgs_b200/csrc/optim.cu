@@ -541,10 +541,10 @@ __global__ void __launch_bounds__(kSmallThreads)
 
 // ----------------------------------------------------------------- AdamW --
 constexpr int kAdamLine = 64;     // elements: whole lines for every type
-// Blocks an SM.  118 M floats, clipped: 4 of them 618 us, 5 (and spills) 632;
-// 150 M bf16 over masters, fewer bytes a thread: 4 823 us, 5 760, 6 834; 1 M
-// masked rows of 59 floats, two vectors under way a thread: 3 162 us, 4 169.
-__host__ __device__ constexpr int adam_resident(bool f32, bool rows) { return rows ? 3 : f32 ? 4 : 5; }
+// Blocks an SM: more have too few registers, fewer too few loads under way
+// (150 M bf16 over masters: 4 743 us, 5 786, 6 879; 118 M floats, clipped: 3
+// 639 us, 4 608, 5 625).
+constexpr int kAdamResident = 4;
 constexpr int kAdamGroups = 32;
 
 struct AdamHyper {
@@ -740,7 +740,6 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
         const int64_t first = (part.lo + L - 1) / L * (L / 4), last = part.hi / 4;
         const int n = int(max(last - first, int64_t(0)));
         const uint32_t skip = uint32_t(4 * first - part.lo);
-        constexpr int kPair = T == 32 ? 1 : 2;
         constexpr int kRowsWarps = T == 32 ? kSmallThreads / 32 : T / 32;
         // Each warp lists the vectors of a stretch that have something to
         // update, and then goes through the list with all lanes at work.
@@ -759,20 +758,12 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
                 count += __popc(some);
             }
             __syncwarp();
-            for (int q = lane; q < count; q += kPair * 32) {
-                typename AdamAt<kF32>::Four x[kPair];
-                int64_t i[kPair];
-                uint32_t keep[kPair];
-#pragma unroll
-                for (int p = 0; p < kPair; ++p) {
-                    const uint32_t entry = q + p * 32 < count ? list[q + p * 32] : 0u;
-                    i[p] = first + base + (entry >> 4);
-                    keep[p] = entry & 15u;
-                    if (keep[p]) at.load(x[p], i[p]);
-                }
-#pragma unroll
-                for (int p = 0; p < kPair; ++p)
-                    if (keep[p]) at.update(x[p], i[p], keep[p]);
+            for (int q = lane; q < count; q += 32) {
+                const uint32_t entry = list[q];
+                const int64_t i = first + base + (entry >> 4);
+                typename AdamAt<kF32>::Four x;
+                at.load(x, i);
+                at.update(x, i, entry & 15u);
             }
             __syncwarp();
         }
@@ -839,7 +830,7 @@ __device__ __forceinline__ void count_update(long long* step) {
 }
 
 template <int N, bool kF32, bool kRows>
-__global__ void __launch_bounds__(kOptThreads, adam_resident(kF32, kRows))
+__global__ void __launch_bounds__(kOptThreads, kAdamResident)
     adamw_kernel(const __grid_constant__ AdamTable<N> tab, const __grid_constant__ AdamCall call) {
     __shared__ double smem[33];
     AdamScale h;
@@ -1224,14 +1215,14 @@ void adamw_all(const xsg_adamw_span* spans, int64_t n, int64_t elems, AdamCall c
     AdamTable<N> tab;
     bool masked = false;
     for (int64_t i = 0; i < n; ++i) masked = masked || spans[i].row_mask;
-    const int32_t tile = tile_for(elems, 1024, masked ? 8192 : 4096, 148 * 4);
+    const int32_t tile = tile_for(elems, 1024, masked ? 8192 : 4096, 148 * kAdamResident);
     bool pdl = call.sums != nullptr;  // the first launch follows the norm's first pass directly
     for (int64_t i = 0; i < n;) {
         bool f32, rows;
         i = fill_adam(tab, spans, i, n, tile, f32, rows);
         call.advance = i >= n;
         call.norm = i >= n ? norm : nullptr;
-        const int blocks = std::max(1, std::min(tab.first[tab.count], 148 * adam_resident(f32, rows)));
+        const int blocks = std::max(1, std::min(tab.first[tab.count], 148 * kAdamResident));
         launch_table(f32 ? (rows ? adamw_kernel<N, true, true> : adamw_kernel<N, true, false>)
                          : (rows ? adamw_kernel<N, false, true> : adamw_kernel<N, false, false>),
                      blocks, kOptThreads, 1, pdl, st, tab, call);
