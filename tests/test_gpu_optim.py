@@ -534,3 +534,124 @@ def test_optimizer_row_masks():
     mask = torch.arange(50, device="cuda") < 20
     opt.step(row_masks={p: mask})
     assert torch.equal(p.detach()[20:], before[20:]) and (p.detach()[:20] != before[:20]).all()
+
+
+def test_optimizer_copies_and_pickles():
+    import copy
+    import pickle
+    p = torch.randn(20, 3, device="cuda", requires_grad=True)
+    opt = X.AdamW([p], lr=0.1, max_norm=2.0)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        q = twin.param_groups[0]["params"][0]
+        assert twin.max_norm == 2.0 and twin._step.tolist() == [1, 0] and q.data_ptr() != p.data_ptr()
+        q.grad = torch.ones_like(q)
+        assert float(twin.step()) > 0 and twin._step.tolist() == [2, 0]
+    assert opt._step.tolist() == [1, 0]
+
+
+# ------------------------------------- each form of a call at its limits --
+@pytest.mark.parametrize("n", [16_383, 16_384, 16_385, 65_537, 262_143, 262_144, 262_145, 600_011, 1_300_003, 2_700_001])
+@pytest.mark.parametrize("tensors", [1, 32, 33])
+def test_every_size_of_call(n, tensors):
+    # one launch, two launches and each size of tile change over between these
+    sizes = [n // (2 * tensors)] * (tensors - 1)
+    sizes.append(n - sum(sizes))
+    p, g, m, v, _ = state_for(sizes, torch.float32, n % 1000)
+    norm = norm64(g, 2)
+    total, each = X.gradient_norm(g, per_tensor=True)
+    assert torch.equal(total, X.gradient_norm(g))
+    assert abs(float(total) - norm) <= 10 * U * norm
+    for got, t in zip(each.tolist(), g):
+        assert abs(got - norm64([t], 2)) <= 10 * U * norm64([t], 2)
+    old = [tuple(x.clone() for x in q) for q in zip(p, g, m, v)]
+    X.adamw_update_(p, g, m, v, X.adamw_step_counter("cuda", 2), lr=0.01, max_norm=0.3 * norm)
+    c = 0.3 * norm / (norm + CLIP_EPS)
+    check_update(p, g, m, v, None, old, 3, [0.01] * tensors, (0.9, 0.999), 1e-8, 0.0, c)
+    before = [t.double() for t in g]
+    X.clip_gradients_(g, 0.3 * norm)
+    for t, b in zip(g, before):
+        assert ((t.double() - b * c).abs() <= 14 * U * (b * c).abs() + TINY[torch.float32]).all()
+
+
+@pytest.mark.parametrize("count", [1, 100, 2047, 2048, 2049, 5000])
+@pytest.mark.parametrize("masked", [False, True])
+def test_adamw_one_launch_or_two(count, masked):
+    p, g, m, v, _ = state_for([count], torch.float32, 7)
+    mask = (torch.arange(count, device="cuda") % 3 == 0) if masked else None
+    old = [tuple(x.clone() for x in q) for q in zip(p, g, m, v)]
+    norm = norm64(g, 2)
+    step = X.adamw_step_counter("cuda", 2)
+    got = X.adamw_update_(p, g, m, v, step, lr=0.01, max_norm=0.3 * norm, row_mask=mask)
+    assert abs(float(got) - norm) <= 10 * U * norm and step.tolist() == [3, 0]
+    check_update(p, g, m, v, None, old, 3, [0.01], (0.9, 0.999), 1e-8, 0.0, 0.3 * norm / (norm + CLIP_EPS),
+                 [mask] if masked else None)
+    before = p[0].clone()
+    g[0][0] = math.nan
+    X.adamw_update_(p, g, m, v, step, lr=0.01, skip_nonfinite=True)
+    assert step.tolist() == [3, 0] and torch.equal(before, p[0])
+
+
+def test_small_calls_in_a_graph():
+    p, g, m, v, _ = state_for([40, 7], torch.float32, 5)
+    step = X.adamw_step_counter("cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        X.adamw_update_(p, g, m, v, step, lr=0.01, max_norm=0.1)
+        X.clip_gradients_(g, 1e9)
+        X.gradient_norm(g, per_tensor=True)
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        X.adamw_update_(p, g, m, v, step, lr=0.01, max_norm=0.1)
+        X.clip_gradients_(g, 1e9)
+        total, each = X.gradient_norm(g, per_tensor=True)
+    for _ in range(4):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert step.tolist() == [5, 0]
+    assert abs(float(total) - norm64(g, 2)) <= 10 * U * norm64(g, 2)
+
+
+def test_large_tensors():
+    n = 52_000_003  # large tiles, more than the L2 holds
+    g = torch.empty(n + 3, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(1))[3:]
+    want = float(torch.linalg.vector_norm(g, dtype=torch.float64))
+    assert abs(float(X.gradient_norm([g])) - want) <= 10 * U * want
+    total, each = X.gradient_norm([g[:7], g[7:]], per_tensor=True)
+    assert abs(float(total) - want) <= 10 * U * want
+    before = g.clone()
+    X.clip_gradients_([g], 0.25 * want)
+    c = 0.25 * want / (want + CLIP_EPS)
+    assert ((g.double() - before.double() * c).abs() <= 14 * U * before.double().abs() * c).all()
+
+
+@pytest.mark.parametrize("m0", [0.0, 1e-45, 1e-41, 1e-3])
+@pytest.mark.parametrize("v0", [0.0, 1e-45, 1e-41, 1e-30, 1e-6, 1e38])
+@pytest.mark.parametrize("eps", [1e-15, 1e-8, 1e-36])
+def test_adamw_subnormal_moments(m0, v0, eps):
+    p = make([3001], torch.float32, 1)
+    g = [torch.zeros(3001, device="cuda")]
+    m, v = [torch.full((3001,), m0, device="cuda")], [torch.full((3001,), v0, device="cuda")]
+    old = [(p[0].clone(), g[0].clone(), m[0].clone(), v[0].clone())]
+    X.adamw_update_(p, g, m, v, X.adamw_step_counter("cuda", 99), lr=1e-3, eps=eps)
+    (w1, m1, v1), (dw, dm, dv) = adamw64(*old[0], 100, 1e-3, (0.9, 0.999), eps, 0.0)
+    assert ((m[0].double().cpu() - m1).abs() <= dm).all() and ((v[0].double().cpu() - v1).abs() <= dv).all()
+    # the update from the 32-bit moments that were written: near the bottom their rounding is part of the inputs
+    mw, vw = m[0].double().cpu(), v[0].double().cpu()
+    scale = 1e-3 / (1 - 0.9 ** 100)
+    den = (vw / (1 - 0.999 ** 100)).sqrt() + eps
+    want = old[0][0].double().cpu() - scale * mw / den
+    bound = 3 * U * (old[0][0].double().cpu().abs() + want.abs()) + 48 * U * scale * mw.abs() / den
+    assert ((p[0].double().cpu() - want).abs() <= bound).all()
+
+
+def test_kinds_of_sequences():
+    ts = make([5, 9000], torch.float32)
+    want = X.gradient_norm(ts)
+    assert torch.equal(X.gradient_norm(tuple(ts)), want) and torch.equal(X.gradient_norm(t for t in ts), want)
+    for bad in (ts[0], 3, [ts[0], None]):
+        with pytest.raises(TypeError, match="grads"):
+            X.gradient_norm(bad)

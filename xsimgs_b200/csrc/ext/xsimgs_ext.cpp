@@ -925,7 +925,9 @@ struct TensorList {
     c10::SmallVector<const Tensor*, 16> at;
 
     TensorList(const py::object& o, const char* name, bool optional = false) {
-        seq = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), name));
+        TORCH_CHECK_TYPE(!THPVariable_Check(o.ptr()), name, " must be a list of tensors, got one tensor");
+        const std::string wanted = std::string(name) + " must be a list of tensors";
+        seq = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), wanted.c_str()));
         if (!seq) throw py::error_already_set();
         const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq.ptr());
         at.reserve(size_t(n));

@@ -144,6 +144,10 @@ class AdamW(torch.optim.Optimizer):
                              masters=masters if any(m is not None for m in masters) else None,
                              row_mask=masks if row_masks else None)
 
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite,
+                "_step": self._step}
+
     def state_dict(self) -> dict:
         d = super().state_dict()
         d["updates"] = 0 if self._step is None else int(self._step[0])
