@@ -628,6 +628,26 @@ def test_large_tensors():
     assert ((g.double() - before.double() * c).abs() <= 14 * U * before.double().abs() * c).all()
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16_master"])
+@pytest.mark.parametrize("clip", [False, True])
+def test_adamw_large(kind, clip):
+    # a block for each tile, behind the norm's own launch
+    sizes = [11_000_001, 3, 9_000_020]
+    p, g, m, v, masters = state_for(sizes, torch.bfloat16 if kind == "bf16_master" else torch.float32, 13,
+                                    masters=kind == "bf16_master")
+    old = [tuple(x.clone() for x in q) for q in zip(masters or p, g, m, v)]
+    norm = norm64(g, 2)
+    step = X.adamw_step_counter("cuda", 2)
+    got = X.adamw_update_(p, g, m, v, step, lr=0.01, masters=masters, max_norm=0.3 * norm if clip else None)
+    check_update(p, g, m, v, masters, old, 3, [0.01] * 3, (0.9, 0.999), 1e-8, 0.0,
+                 0.3 * norm / (norm + CLIP_EPS) if clip else 1.0)
+    assert step.tolist() == [3, 0] and (not clip or abs(float(got) - norm) <= 10 * U * norm)
+    g[0][5_000_000] = math.nan
+    before = [x.clone() for x in p]
+    X.adamw_update_(p, g, m, v, step, lr=0.01, masters=masters, skip_nonfinite=True)
+    assert step.tolist() == [3, 0] and all(torch.equal(a, b) for a, b in zip(p, before))
+
+
 @pytest.mark.parametrize("m0", [0.0, 1e-45, 1e-41, 1e-3])
 @pytest.mark.parametrize("v0", [0.0, 1e-45, 1e-41, 1e-30, 1e-6, 1e38])
 @pytest.mark.parametrize("eps", [1e-15, 1e-8, 1e-36])
