@@ -29,6 +29,12 @@ def lib() -> C.CDLL:
         _lib.xsg_rasterize_workspace_size.argtypes = [C.c_int64, C.c_int, C.c_int64, C.c_int64, C.c_int]
         _lib.xsg_sh_bwd_workspace_size.restype = C.c_size_t
         _lib.xsg_sh_bwd_workspace_size.argtypes = [C.c_int64]
+        _lib.xsg_grad_norm_workspace_size.restype = C.c_size_t
+        _lib.xsg_grad_norm_workspace_size.argtypes = [C.c_int64]
+        for f in (_lib.xsg_grad_norm_workspace_bytes, _lib.xsg_clip_grads_workspace_bytes,
+                  _lib.xsg_adamw_workspace_bytes):
+            f.restype = C.c_size_t
+            f.argtypes = [C.c_void_p, C.c_int64]
         _lib.xsg_timing_query.argtypes = [C.c_char_p, C.POINTER(C.c_double), C.POINTER(C.c_longlong)]
         _lib.xsg_fp32_probe.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.POINTER(C.c_double)]
         _lib.xsg_set_pair_counters.argtypes = [C.c_void_p]

@@ -18,9 +18,9 @@
 // first one ends and starts at the tiles that the first one read last.
 //
 // Measured on B200, 6449 GB/s being a copy's rate: norm of 640 M floats
-// 351 us (7290 GB/s), of 160 M bf16 51 us (6220); clipping 118 M floats 236 us
-// (its three passes of 472 MB less 76 MB that the L2 still holds: 5680); the
-// clipped update of 118 M floats 589 us (3304 MB and the norm's 472: 6410), of
+// 351 us (7290 GB/s), of 160 M bf16 51 us (6220); clipping 118 M floats 227 us
+// (its three passes of 472 MB: 6240, of which the L2 serves some); the
+// clipped update of 118 M floats 585 us (3304 MB and the norm's 472: 6450), of
 // 150 M bf16 over masters 738 us (4.5 GB: 6100), of 35 % of 1 M rows of 59
 // floats 166 us.
 #include <cooperative_groups.h>
@@ -168,8 +168,9 @@ __device__ __forceinline__ void add16(double& acc, const float (&x)[16]) {
 }
 
 // Sum (or maximum) over the numbers [lo, hi) of a tensor, by a team of T
-// threads (a block or a warp) of which this is number `me`.
-template <int P, int D, int T>
+// threads (a block or a warp) of which this is number `me`.  kEarly: the data
+// need not stay in the L2.
+template <int P, int D, int T, bool kEarly>
 __device__ __forceinline__ double reduce_part(const void* base, Part part, int me) {
     constexpr int V = 16 / elem_size(D);  // elements of a vector
     constexpr int kUnroll = 4;
@@ -216,7 +217,7 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part, int m
     for (; i + (kUnroll - 1) * T < n; i += kUnroll * T) {
         uint4 q[kUnroll];
 #pragma unroll
-        for (int k = 0; k < kUnroll; ++k) q[k] = vec[i + k * T];
+        for (int k = 0; k < kUnroll; ++k) q[k] = kEarly ? __ldcs(vec + i + k * T) : vec[i + k * T];
         take(q);
     }
     if (i < n) {
@@ -240,12 +241,12 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part, int m
     return acc;
 }
 
-template <int P, int T, typename Table>
+template <int P, int T, bool kEarly = false, typename Table>
 __device__ __forceinline__ double reduce_part(const Table& tab, int t, Part part, int me) {
     const int dtype = tab.dtype[t];
-    if (dtype == XSG_F32) return reduce_part<P, XSG_F32, T>(tab.base[t], part, me);
-    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16, T>(tab.base[t], part, me);
-    return reduce_part<P, XSG_F16, T>(tab.base[t], part, me);
+    if (dtype == XSG_F32) return reduce_part<P, XSG_F32, T, kEarly>(tab.base[t], part, me);
+    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16, T, kEarly>(tab.base[t], part, me);
+    return reduce_part<P, XSG_F16, T, kEarly>(tab.base[t], part, me);
 }
 
 // Over the block, in a fixed order; every thread gets the result.  `smem`
@@ -275,7 +276,12 @@ __device__ __forceinline__ float clip_coefficient(float norm, float max_norm) {
 }
 
 // Partial sums of a launch: sums[b] of all tiles of block b, which takes them
-// in turn.
+// in turn.  What comes before the last 80 MB is read as data that need not
+// stay in the L2 (clipping 118 M floats: 236 us without, 227.5 with 64 to 120
+// MB; the second pass finds as much in the L2 as before, 76 MB, so what gains
+// is the write-back of the lines that the pass before has left there).
+constexpr int64_t kKeptBytes = int64_t(80) << 20;
+
 template <int P, int N>
 __global__ void __launch_bounds__(kOptThreads, kNormResident)
     norm_partial_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums) {
@@ -287,7 +293,11 @@ __global__ void __launch_bounds__(kOptThreads, kNormResident)
     for (int32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         if (t < 0) t = owner_of(tab, tile);
         while (tile >= tab.first[t + 1]) ++t;
-        acc = join<P>(acc, reduce_part<P, kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), threadIdx.x));
+        const Part part = part_of(tab, t, tile, tile + 1);
+        if (int64_t(tiles - tile) * tab.tile_bytes > kKeptBytes)
+            acc = join<P>(acc, reduce_part<P, kOptThreads, true>(tab, t, part, threadIdx.x));
+        else
+            acc = join<P>(acc, reduce_part<P, kOptThreads>(tab, t, part, threadIdx.x));
     }
     acc = block_reduce<P>(acc, smem);
     if (threadIdx.x == 0) sums[blockIdx.x] = acc;
@@ -305,14 +315,22 @@ __global__ void __launch_bounds__(kOptThreads, kNormResident)
     pdl_trigger();
     const int32_t tiles = tab.first[tab.count], end = run_start(tiles, gridDim.x, blockIdx.x + 1);
     int32_t tile = run_start(tiles, gridDim.x, blockIdx.x);
+    // no second pass follows (largest entry of 160 M bf16: 54.8 us, 56.4 without)
+    const bool early = int64_t(tiles) * tab.tile_bytes > kKeptBytes;
     double whole = 0.0;
     for (int t = owner_of(tab, tile); tile < end; ++t) {
         const int32_t stop = min(end, tab.first[t + 1]);
         if (stop <= tile) continue;
         // tile by tile, so that the same entries meet in 32 bits as in the kernel above
         double acc = 0.0;
-        for (; tile < stop; ++tile)
-            acc = join<P>(acc, reduce_part<P, kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), threadIdx.x));
+        if (early) {
+            for (; tile < stop; ++tile)
+                acc = join<P>(acc, reduce_part<P, kOptThreads, true>(tab, t, part_of(tab, t, tile, tile + 1),
+                                                                     threadIdx.x));
+        } else {
+            for (; tile < stop; ++tile)
+                acc = join<P>(acc, reduce_part<P, kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), threadIdx.x));
+        }
         acc = block_reduce<P>(acc, smem);
         if (threadIdx.x == 0) slots[blockIdx.x + t] = acc;
         whole = join<P>(whole, acc);
@@ -987,8 +1005,8 @@ struct SpanLaunch {
         return int32_t(tiles);
     }
     void close(int64_t& sums, int64_t& slots) {
-        // from 16 KB on, larger tiles only where each block has many (118 M floats: 32 KB 236 us to clip, 16 KB 238,
-        // 64 KB 240)
+        // from 16 KB on, larger tiles only where each block has many (clipping 118 M floats: 16 KB 238 us,
+        // 32 KB 236, 64 KB 240)
         const bool many = bytes > (int64_t(32) << 10) * kOptBlocks * 8;
         blocks = std::max(1, std::min(cut(many ? 32768 : tile_for(bytes, 4096, 16384, kOptBlocks)), kOptBlocks));
         sums_at = sums;
