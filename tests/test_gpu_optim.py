@@ -675,3 +675,34 @@ def test_kinds_of_sequences():
     for bad in (ts[0], 3, [ts[0], None]):
         with pytest.raises(TypeError, match="grads"):
             X.gradient_norm(bad)
+
+
+def test_views_that_negate():
+    z = torch.randn(500, dtype=torch.complex64, device="cuda").conj()
+    neg = z.imag  # a float view with the sign to be turned
+    assert neg.is_neg()
+    p, g, m, v, _ = state_for([500], torch.float32, 3)
+    g = [neg]
+    old = [(p[0].clone(), neg.clone(), m[0].clone(), v[0].clone())]
+    X.adamw_update_(p, g, m, v, X.adamw_step_counter("cuda"), lr=0.01)
+    check_update(p, g, m, v, None, old, 1, [0.01], (0.9, 0.999), 1e-8, 0.0)
+    with pytest.raises(RuntimeError, match="negate|dense"):
+        X.clip_gradients_([neg], 1.0)
+
+
+def test_instrumentation():
+    from xsimgs_b200 import capi
+    p, g, m, v, _ = state_for([70_000], torch.float32, 3)
+    step = X.adamw_step_counter("cuda")
+    before = capi.launch_count()
+    capi.timing_reset()
+    capi.timing_enable(True)
+    X.gradient_norm(g)
+    X.clip_gradients_(g, 1e-3)
+    X.adamw_update_(p, g, m, v, step, lr=0.1, max_norm=1.0)
+    capi.timing_enable(False)
+    assert capi.launch_count() - before == 1 + 2 + 2
+    for name in ("grad_norm", "clip_grads", "adamw_update"):
+        ms, count = capi.timing_query(name)
+        assert count == 1 and 0 < ms < 100
+    capi.timing_reset()

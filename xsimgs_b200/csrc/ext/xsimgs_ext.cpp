@@ -988,6 +988,7 @@ void check_listed(const Tensor& t, const char* name, const Tensor& ref) {
 // of its own, without gaps.
 void check_written(const Tensor& t, const char* name, const Tensor& ref) {
     check_listed(t, name, ref);
+    TORCH_CHECK(!t.is_neg(), name, " must not be views that negate");
     TORCH_CHECK(t.is_non_overlapping_and_dense(), name, " must be dense (no gaps, no expanded dimensions): got sizes ",
                 t.sizes(), " with strides ", t.strides());
 }
@@ -1130,7 +1131,7 @@ std::optional<Tensor> adamw_update(const py::object& params_seq, const py::objec
                 "adamw_update_: step must be a contiguous int64 tensor of two words (adamw_step_counter)");
     c10::cuda::CUDAGuard g(params[0].device());
     c10::SmallVector<xsg_adamw_span, 16> spans(n);
-    std::vector<Tensor> copies;  // of gradients whose order of dimensions is not their parameter's
+    std::vector<Tensor> copies;  // of gradients whose order of dimensions is not their parameter's, or that negate
     Extents extents;
     extents.reserve(5 * n + 1);
     add_extent(extents, step, true);
@@ -1154,7 +1155,7 @@ std::optional<Tensor> adamw_update(const py::object& params_seq, const py::objec
                     " and ", p.sizes());
         s.grad_dtype = dtype_code(grads[i], "grads");
         s.param_dtype = dtype_code(p, "params");
-        const bool same = same_order(grads[i], p);
+        const bool same = same_order(grads[i], p) && !grads[i].is_neg();
         if (!same) copies.push_back(at::empty_strided(p.sizes(), p.strides(), grads[i].options()).copy_(grads[i]));
         const Tensor& grad = same ? grads[i] : copies.back();
         add_extent(extents, p, true);

@@ -1140,6 +1140,7 @@ int grad_norm(const xsg_span* spans, int64_t n, int norm_type, float* norm, floa
     if (arena.cap < xsg_grad_norm_workspace_bytes(spans, n))
         return set_error(XSG_ERR_WORKSPACE, "grad_norm: workspace too small");
     const auto get = [&](int64_t i, auto& L) { L.add(spans[i].data, spans[i].n, spans[i].dtype); };
+    ScopedTimer tm("grad_norm", st);
     const int rc = with_plan(n, get, [&](const auto& plan) {
         return with_norm_type(norm_type, "grad_norm",
                               [&](auto p) { return norm_all<decltype(p)::value>(plan, norm, norms, arena, n, st); });
@@ -1155,6 +1156,7 @@ int clip_grads(const xsg_span* spans, int64_t n, int norm_type, float max_norm, 
     if (arena.cap < xsg_clip_grads_workspace_bytes(spans, n))
         return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
     const auto get = [&](int64_t i, auto& L) { L.add(spans[i].data, spans[i].n, spans[i].dtype); };
+    ScopedTimer tm("clip_grads", st);
     const int rc = with_plan(n, get, [&](const auto& plan) {
         return with_norm_type(norm_type, "clip_grads",
                               [&](auto p) { return clip_all<decltype(p)::value>(plan, max_norm, norm, arena, n, st); });
@@ -1283,6 +1285,7 @@ int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float ma
     if (int rc = check_adamw(spans, n)) return rc;
     XSG_REQUIRE(step, "adamw_update: null step counter");
     XSG_REQUIRE(max_norm < 0.f || std::isfinite(max_norm), "adamw_update: max_norm must be finite");
+    ScopedTimer tm("adamw_update", st);
     AdamCall call{};
     call.step = reinterpret_cast<long long*>(step);
     call.clip = max_norm >= 0.f;
