@@ -11,18 +11,19 @@
 // first 4 again, where the L2 has lost them) for the scaling, 28 for the
 // update.  The tensors travel as a table in the kernel's parameters, so that
 // a call copies nothing to the device and can be captured in a graph.  Each
-// tensor is cut into tiles, and blocks (of small tensors, warps) take the
-// tiles of all tensors in turn, so that tensors of any size share the work
-// evenly.  The order of every sum depends on the tensors' sizes and offsets
-// alone: the same bits on every run.  A second pass is launched while the
-// first one ends and starts at the tiles that the first one read last.
+// tensor is cut into tiles.  Blocks (of small tensors, warps) take the tiles
+// of all tensors in turn where they are summed, so that the order of every sum
+// depends on the tensors' sizes and offsets alone: the same bits on every run.
+// Where they are written, blocks fetch them from a counter.  A second pass is
+// launched while the first one ends and starts at the tiles that the first one
+// read last.
 //
 // Measured on B200, 6449 GB/s being a copy's rate: norm of 640 M floats
-// 351 us (7290 GB/s), of 160 M bf16 51 us (6220); clipping 118 M floats 227 us
-// (its three passes of 472 MB: 6240, of which the L2 serves some); the
-// clipped update of 118 M floats 585 us (3304 MB and the norm's 472: 6450), of
-// 150 M bf16 over masters 738 us (4.5 GB: 6100), of 35 % of 1 M rows of 59
-// floats 166 us.
+// 351 us (7290 GB/s), of 160 M bf16 51 us (6220); clipping 118 M floats 214 us
+// (its three passes of 472 MB: 6620, of which the L2 serves some); the
+// clipped update of 118 M floats 571 us (3304 MB and the norm's 472: 6610), of
+// 150 M bf16 over masters 699 us (4.5 GB: 6440), of 35 % of 1 M rows of 59
+// floats 158 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -284,9 +285,11 @@ constexpr int64_t kKeptBytes = int64_t(80) << 20;
 
 template <int P, int N>
 __global__ void __launch_bounds__(kOptThreads, kNormResident)
-    norm_partial_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums) {
+    norm_partial_kernel(const __grid_constant__ SpanTable<N> tab, double* __restrict__ sums,
+                        unsigned* __restrict__ fetched) {
     __shared__ double smem[33];
     pdl_trigger();
+    if (fetched && blockIdx.x == 0 && threadIdx.x == 0) *fetched = 0;  // for the second pass
     const int32_t tiles = tab.first[tab.count];
     double acc = 0.0;
     int t = -1;
@@ -427,23 +430,35 @@ __device__ __forceinline__ void scale_part(const Table& tab, int t, Part part, f
 }
 
 // The second pass of clipping.  c = 1 leaves the data alone.  The tiles are
-// taken from the last to the first, so that what the first pass read last,
-// and the L2 still holds, comes first.
+// taken from the last to the first, so that what the first pass read last, and
+// the L2 still holds, comes first.  A block fetches the next tile while it
+// works on one: the reads and writes then go through the memory in order,
+// with the blocks out of step, which HBM likes better than blocks that take
+// every 592nd tile (clipping 118 M floats: 214 us against 227, 90 M bf16 78.9
+// against 80.9) or a block for each tile (216.5, and 4 us more where nothing
+// has to be scaled).  Which block has which tile changes no result.
 template <int P, int N>
 __global__ void __launch_bounds__(kOptThreads, kScaleResident)
     clip_scale_kernel(const __grid_constant__ SpanTable<N> tab, const double* sums, int n_sums,
-                      float max_norm, float* __restrict__ norm) {
+                      float max_norm, float* __restrict__ norm, unsigned* fetched) {
     __shared__ double smem[33];
+    __shared__ int32_t next[2];
     pdl_wait();
     const float total = total_norm<P>(sums, n_sums, smem);
     if (blockIdx.x == 0 && threadIdx.x == 0 && norm) *norm = total;
     const float c = clip_coefficient(total, max_norm);
     if (c == 1.f) return;
+    const int32_t tiles = tab.first[tab.count];
+    if (threadIdx.x == 0) next[0] = int32_t(atomicAdd(fetched, 1u));
+    __syncthreads();
     int t = -1;
-    for (int32_t tile = tab.first[tab.count] - 1 - int32_t(blockIdx.x); tile >= 0; tile -= gridDim.x) {
+    for (int turn = 0; next[turn] < tiles; turn ^= 1) {
+        const int32_t tile = tiles - 1 - next[turn];
+        if (threadIdx.x == 0) next[turn ^ 1] = int32_t(atomicAdd(fetched, 1u));
         if (t < 0) t = owner_of(tab, tile);
         while (tile < tab.first[t]) --t;
         scale_part<kOptThreads>(tab, t, part_of(tab, t, tile, tile + 1), c, threadIdx.x);
+        __syncthreads();
     }
 }
 
@@ -573,14 +588,18 @@ __global__ void __launch_bounds__(kSmallThreads)
 }
 
 // ----------------------------------------------------------------- AdamW --
-// Bound by HBM: 16 bytes a lane from each of four arrays are under way in four
+// Bound by HBM: 16 bytes a lane from each of four arrays are under way in five
 // blocks an SM.  Moments and arithmetic are in 32 bits; w is rounded once to a
 // 16-bit parameter's type.
 constexpr int kAdamLine = 64;     // elements: whole lines for every type
 // Blocks an SM: more have too few registers, fewer too few loads under way
-// (150 M bf16 over masters: 4 743 us, 5 786, 6 879; 118 M floats, clipped: 3
-// 639 us, 4 608, 5 625).
-constexpr int kAdamResident = 4;
+// (150 M bf16 over masters: 4 728 us, 5 699, 6 737; 118 M floats, clipped: 3
+// 610 us, 4 574, 5 571, 6 608; 1 M masked rows: 4 171 us, 5 158, 6 161).
+constexpr int kAdamResident = 5;
+// Elements of a tile at most: without row masks (150 M bf16 over masters: 4096
+// 699 us, 8192 710), and with them, where each of a block's eight warps goes
+// through a stretch of 1024 (1 M masked rows: 4096 201 us, 8192 158, 16384 171).
+constexpr int32_t kAdamTile = 4096, kRowsTile = 8192;
 constexpr int kAdamGroups = 32;
 
 struct AdamHyper {
@@ -616,9 +635,8 @@ struct AdamTable {
 };
 
 struct AdamCall {
-    long long* step;      // [0] updates taken, [1] blocks that are done (zero between launches)
-    const double* sums;   // the gradients' partial sums, or null
-    const float* total;   // or their norm, or null
+    unsigned long long* step;  // [0] updates taken, [1] tiles fetched (zero between launches)
+    const double* sums;        // the gradients' partial sums, or null
     int32_t n_sums;
     int32_t advance;      // the call's last launch counts the update
     int32_t clip;
@@ -832,55 +850,61 @@ __device__ __forceinline__ void adam_part(const AdamEntry& e, Part part, const A
     }
 }
 
-// The tiles of team b of `teams`, in turn (a part of a masked tensor may
-// have little to do) and from the last to the first, as in clipping.
+// The options of a tensor's group at this step.
+__device__ __forceinline__ void set_group(AdamScale& h, const AdamHyper& y, float steps) {
+    h.beta1 = y.beta1, h.rest1 = y.rest1, h.beta2 = y.beta2, h.rest2 = y.rest2;
+    h.lr_decay = y.lr_decay, h.eps = y.eps;
+    // 1 - b^t without the cancellation of 1 - pow(b, t)
+    h.step_size = y.lr / -expm1f(steps * y.log_beta1);
+    h.root_scale = rsqrtf(-expm1f(steps * y.log_beta2));
+}
+
+// One tile of tensor t, by a team of T threads.
 template <bool kF32, bool kRows, int T, typename Table>
-__device__ __forceinline__ void adam_tiles(const Table& tab, int32_t b, int32_t teams, int me, float steps, AdamScale& h) {
-    int t = -1;
-    for (int32_t tile = tab.first[tab.count] - 1 - b; tile >= 0; tile -= teams) {
-        if (t < 0 || tile < tab.first[t]) {
-            if (t < 0) t = owner_of(tab, tile);
-            while (tile < tab.first[t]) --t;
-            const AdamHyper& y = tab.hyper[tab.entry[t].group];
-            h.beta1 = y.beta1, h.rest1 = y.rest1, h.beta2 = y.beta2, h.rest2 = y.rest2;
-            h.lr_decay = y.lr_decay, h.eps = y.eps;
-            // 1 - b^t without the cancellation of 1 - pow(b, t)
-            h.step_size = y.lr / -expm1f(steps * y.log_beta1);
-            h.root_scale = rsqrtf(-expm1f(steps * y.log_beta2));
-        }
-        const AdamEntry& e = tab.entry[t];
-        const int64_t at = int64_t(tile - tab.first[t]) * tab.tile;
-        adam_part<kF32, kRows, T>(e, {max(int64_t(e.lead), at), min(e.end, at + tab.tile)}, h, me);
-    }
+__device__ __forceinline__ void adam_tile(const Table& tab, int t, int32_t tile, const AdamScale& h, int me) {
+    const AdamEntry& e = tab.entry[t];
+    const int64_t at = int64_t(tile - tab.first[t]) * tab.tile;
+    adam_part<kF32, kRows, T>(e, {max(int64_t(e.lead), at), min(e.end, at + tab.tile)}, h, me);
 }
 
-// The last of the blocks to come counts the update: all have read step[0] by then.
-__device__ __forceinline__ void count_update(long long* step) {
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        auto* word = reinterpret_cast<unsigned long long*>(step);
-        if (atomicAdd(word + 1, 1ull) == gridDim.x - 1) {
-            word[0] += 1;
-            word[1] = 0;
-        }
-    }
-}
-
+// Blocks fetch tiles as in clipping, from the last to the first.  Every block
+// fetches one past the last; the last of them to do so leaves the counter at
+// zero and counts the update, when all blocks that have had a tile have long
+// read step[0].
 template <int N, bool kF32, bool kRows>
 __global__ void __launch_bounds__(kOptThreads, kAdamResident)
     adamw_kernel(const __grid_constant__ AdamTable<N> tab, const __grid_constant__ AdamCall call) {
     __shared__ double smem[33];
+    __shared__ uint64_t next[2];
     AdamScale h;
     h.c = 1.f;
-    if (call.sums || call.total) {
+    if (call.sums) {
         pdl_wait();
-        const float total = call.total ? __ldcg(call.total) : total_norm<2>(call.sums, call.n_sums, smem);
+        const float total = total_norm<2>(call.sums, call.n_sums, smem);
         if (blockIdx.x == 0 && threadIdx.x == 0 && call.norm) *call.norm = total;
         if (call.skip_nonfinite && !isfinite(total)) return;  // every block alike: nothing changes
         if (call.clip) h.c = clip_coefficient(total, call.max_norm);
     }
-    adam_tiles<kF32, kRows, kOptThreads>(tab, blockIdx.x, gridDim.x, threadIdx.x, float(call.step[0] + 1), h);
-    if (call.advance) count_update(call.step);
+    const float steps = float(call.step[0] + 1);
+    const uint32_t tiles = uint32_t(tab.first[tab.count]);
+    if (threadIdx.x == 0) next[0] = atomicAdd(call.step + 1, 1ull);
+    __syncthreads();
+    int t = -1, turn = 0;
+    for (; next[turn] < tiles; turn ^= 1) {
+        const int32_t tile = int32_t(tiles - 1u - uint32_t(next[turn]));
+        if (threadIdx.x == 0) next[turn ^ 1] = atomicAdd(call.step + 1, 1ull);
+        if (t < 0 || tile < tab.first[t]) {
+            if (t < 0) t = owner_of(tab, tile);
+            while (tile < tab.first[t]) --t;
+            set_group(h, tab.hyper[tab.entry[t].group], steps);
+        }
+        adam_tile<kF32, kRows, kOptThreads>(tab, t, tile, h, threadIdx.x);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0 && next[turn] == uint64_t(tiles) + gridDim.x - 1) {
+        if (call.advance) call.step[0] += 1;
+        call.step[1] = 0;
+    }
 }
 
 // Norm and update of small tensors in one launch (see norm_small_kernel).
@@ -898,7 +922,12 @@ __global__ void __launch_bounds__(kSmallThreads)
     AdamScale h;
     h.c = call.clip ? clip_coefficient(total, call.max_norm) : 1.f;
     const Worker w = worker_of(cluster);
-    adam_tiles<kF32, true, 32>(tab, w.id, w.count, w.lane, steps, h);
+    int group_of = -1;
+    for_tiles(tab, w.id, w.count, [&](int t, int32_t tile) {
+        if (t != group_of) set_group(h, tab.hyper[tab.entry[t].group], steps);
+        group_of = t;
+        adam_tile<kF32, true, 32>(tab, t, tile, h, w.lane);
+    });
     if (first) call.step[0] += 1;  // all have read it before the norm's barriers
 }
 
@@ -922,7 +951,7 @@ bool small_norm(int64_t n_spans, int64_t bytes) { return n_spans <= kSmallSpans 
 bool small_clip(int64_t n_spans, int64_t bytes) { return n_spans <= kSmallSpans && bytes <= kSmallClipBytes; }
 bool small_adamw(int64_t n_spans, int64_t elems) { return n_spans <= kSmallSpans && elems <= kSmallAdamElems; }
 
-// The smallest tile that leaves a block one, up to `most`.
+// The smallest tile that leaves each block one, up to `most`.
 int32_t tile_for(int64_t size, int32_t least, int32_t most, int64_t blocks) {
     while (least < most && size > least * blocks) least *= 2;
     return least;
@@ -1040,14 +1069,15 @@ struct SpanPlan {
     int64_t bytes() const { return launches[0].bytes; }
 
     template <int P>
-    void partials(double* sums_at, double* slots_at, cudaStream_t st) const {
-        for (const auto& L : launches) {
+    void partials(double* sums_at, double* slots_at, unsigned* fetched, cudaStream_t st) const {
+        for (size_t l = 0; l < launches.size(); ++l) {
+            const auto& L = launches[l];
             if (slots_at)
                 launch_table(norm_partial_each_kernel<P, N>, L.blocks, kOptThreads, 1, false, st, L.tab,
                              sums_at + L.sums_at, slots_at + L.slots_at);
             else
                 launch_table(norm_partial_kernel<P, N>, L.blocks, kOptThreads, 1, false, st, L.tab,
-                             sums_at + L.sums_at);
+                             sums_at + L.sums_at, fetched ? fetched + l : nullptr);
         }
     }
 };
@@ -1086,7 +1116,7 @@ int norm_all(const SpanPlan<N>& plan, float* norm, float* norms, Arena arena, in
     }
     double* sums = arena.take<double>(sums_count(n));
     double* slots = norms ? arena.take<double>(slots_count(n)) : nullptr;
-    plan.template partials<P>(sums, slots, st);
+    plan.template partials<P>(sums, slots, nullptr, st);
     for (size_t l = 0; l < plan.launches.size(); ++l) {
         const SpanLaunch<N>& L = plan.launches[l];
         const bool last = l + 1 == plan.launches.size();
@@ -1108,10 +1138,11 @@ int clip_all(const SpanPlan<N>& plan, float max_norm, float* norm, Arena arena, 
         }
     }
     double* sums = arena.take<double>(sums_count(n));
-    plan.template partials<P>(sums, nullptr, st);
+    unsigned* fetched = arena.take<unsigned>(plan.launches.size());
+    plan.template partials<P>(sums, nullptr, fetched, st);
     for (size_t l = plan.launches.size(); l-- > 0;)
         launch_table(clip_scale_kernel<P, N>, std::min(plan.launches[l].blocks, 148 * kScaleResident), kOptThreads, 1, l + 1 == plan.launches.size(),
-                     st, plan.launches[l].tab, sums, int(plan.sums), max_norm, l == 0 ? norm : nullptr);
+                     st, plan.launches[l].tab, sums, int(plan.sums), max_norm, l == 0 ? norm : nullptr, fetched + l);
     return XSG_OK;
 }
 
@@ -1261,21 +1292,21 @@ int64_t fill_adam(AdamTable<N>& tab, const xsg_adamw_span* spans, int64_t i, int
 }
 
 template <int N>
-void adamw_all(const xsg_adamw_span* spans, int64_t n, int64_t elems, AdamCall call, float* norm, bool each_tile,
-               bool masked, cudaStream_t st) {
+void adamw_all(const xsg_adamw_span* spans, int64_t n, int64_t elems, AdamCall call, float* norm, cudaStream_t st) {
     AdamTable<N> tab;
-    const int32_t most = masked || elems > (int64_t(8192) * 148 * kAdamResident * 4) ? 8192 : 4096;
-    const int32_t tile = most == 8192 && !masked ? 8192 : tile_for(elems, 1024, most, 148 * kAdamResident);
-    bool pdl = call.sums || call.total;  // the first launch follows the norm's directly
+    bool masked = false;
+    for (int64_t i = 0; i < n; ++i) masked = masked || spans[i].row_mask;
+    const int32_t tile = tile_for(elems, 1024, masked ? kRowsTile : kAdamTile, 148 * kAdamResident);
+    bool pdl = call.sums != nullptr;  // the first launch follows the norm's directly
     for (int64_t i = 0; i < n;) {
         bool f32, rows;
         i = fill_adam(tab, spans, i, n, tile, f32, rows);
         call.advance = i >= n;
         call.norm = i >= n ? norm : nullptr;
-        const int32_t tiles = std::max(1, tab.first[tab.count]);
+        const int blocks = std::max(1, std::min(tab.first[tab.count], 148 * kAdamResident));
         launch_table(f32 ? (rows ? adamw_kernel<N, true, true> : adamw_kernel<N, true, false>)
                          : (rows ? adamw_kernel<N, false, true> : adamw_kernel<N, false, false>),
-                     each_tile ? tiles : std::min(tiles, 148 * kAdamResident), kOptThreads, 1, pdl, st, tab, call);
+                     blocks, kOptThreads, 1, pdl, st, tab, call);
         pdl = false;
     }
 }
@@ -1287,27 +1318,15 @@ int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float ma
     XSG_REQUIRE(max_norm < 0.f || std::isfinite(max_norm), "adamw_update: max_norm must be finite");
     ScopedTimer tm("adamw_update", st);
     AdamCall call{};
-    call.step = reinterpret_cast<long long*>(step);
+    call.step = reinterpret_cast<unsigned long long*>(step);
     call.clip = max_norm >= 0.f;
     call.skip_nonfinite = skip_nonfinite;
     call.max_norm = max_norm;
     int64_t elems = 0;
-    bool masked = false;
-    for (int64_t i = 0; i < n; ++i) {
-        elems += spans[i].n;
-        masked = masked || spans[i].row_mask;
-    }
-    // A block for each tile leaves the order of the reads and writes to the
-    // block scheduler, which HBM likes better than blocks in step (118 M
-    // floats: 498 us against 535, 24 M 109 against 114); under row masks the
-    // blocks that stay balance better (1 M rows, 35 % seen: 166 us against
-    // 181).  Behind a norm it takes a launch that adds up the partial sums,
-    // worth it for many tiles.
-    const bool normed = call.clip || skip_nonfinite || norm;
-    const bool each_tile = !masked && (!normed || elems >= int64_t(1) << 24);
+    for (int64_t i = 0; i < n; ++i) elems += spans[i].n;
     int rc = XSG_OK;
     bool done = false;
-    if (normed) {
+    if (call.clip || skip_nonfinite || norm) {
         if (arena.cap < xsg_adamw_workspace_bytes(spans, n))
             return set_error(XSG_ERR_WORKSPACE, "adamw_update: workspace too small");
         const auto get = [&](int64_t i, auto& L) { L.add(spans[i].grad, spans[i].n, spans[i].grad_dtype); };
@@ -1326,24 +1345,16 @@ int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float ma
                 }
             }
             double* sums = arena.take<double>(sums_count(n));
-            plan.template partials<2>(sums, nullptr, st);
-            if (each_tile) {
-                // one block adds the sums up for all
-                float* total = arena.take<float>(1);
-                const auto& last = plan.launches.back();
-                launch_norm_finish<2>(last, sums, int(plan.sums), nullptr, total, nullptr, true, st);
-                call.total = total;
-            } else {
-                call.sums = sums;
-                call.n_sums = int(plan.sums);
-            }
+            plan.template partials<2>(sums, nullptr, nullptr, st);
+            call.sums = sums;
+            call.n_sums = int(plan.sums);
             return int(XSG_OK);
         });
     }
     if (rc) return rc;
     if (!done) {
-        if (n <= kSmallSpans) adamw_all<kSmallSpans>(spans, n, elems, call, norm, each_tile, masked, st);
-        else adamw_all<kAdamSpans>(spans, n, elems, call, norm, each_tile, masked, st);
+        if (n <= kSmallSpans) adamw_all<kSmallSpans>(spans, n, elems, call, norm, st);
+        else adamw_all<kAdamSpans>(spans, n, elems, call, norm, st);
     }
     return check_launch("adamw_update");
 }
