@@ -19,8 +19,8 @@
 // read last.
 //
 // Measured on B200, 6449 GB/s being a copy's rate: norm of 640 M floats
-// 351 us (7290 GB/s), of 160 M bf16 51 us (6220); clipping 118 M floats 214 us
-// (its three passes of 472 MB: 6620, of which the L2 serves some); the
+// 351 us (7290 GB/s), of 160 M bf16 51 us (6220); clipping 118 M floats 213 us
+// (its three passes of 472 MB: 6650, of which the L2 serves some); the
 // clipped update of 118 M floats 571 us (3304 MB and the norm's 472: 6610), of
 // 150 M bf16 over masters 699 us (4.5 GB: 6440), of 35 % of 1 M rows of 59
 // floats 158 us.
@@ -79,13 +79,16 @@ __device__ __forceinline__ void store_as(void* p, int dtype, int64_t i, float x)
 // [first[t], first[t + 1]) of the launch.
 constexpr int kLine = 128;
 
+struct SpanEntry {
+    void* base;
+    int64_t end;
+    uint8_t lead, dtype;
+};
+
 template <int N>
 struct SpanTable {
-    void* base[N];
-    int64_t end[N];
+    SpanEntry entry[N];
     int32_t first[N + 1];
-    uint8_t lead[N];
-    uint8_t dtype[N];
     int32_t count;
     int32_t tile_bytes;
 };
@@ -96,8 +99,9 @@ struct Part {
 };
 template <typename Table>
 __device__ __forceinline__ Part part_of(const Table& tab, int t, int32_t tile, int32_t stop) {
-    const int64_t per = tab.tile_bytes / elem_size(tab.dtype[t]);
-    return {max(int64_t(tab.lead[t]), (tile - tab.first[t]) * per), min(tab.end[t], (stop - tab.first[t]) * per)};
+    const SpanEntry& e = tab.entry[t];
+    const int64_t per = tab.tile_bytes >> (e.dtype == XSG_F32 ? 2 : 1);
+    return {max(int64_t(e.lead), (tile - tab.first[t]) * per), min(e.end, (stop - tab.first[t]) * per)};
 }
 
 // The contiguous run of tiles of block b out of `blocks`, and the block whose
@@ -244,10 +248,10 @@ __device__ __forceinline__ double reduce_part(const void* base, Part part, int m
 
 template <int P, int T, bool kEarly = false, typename Table>
 __device__ __forceinline__ double reduce_part(const Table& tab, int t, Part part, int me) {
-    const int dtype = tab.dtype[t];
-    if (dtype == XSG_F32) return reduce_part<P, XSG_F32, T, kEarly>(tab.base[t], part, me);
-    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16, T, kEarly>(tab.base[t], part, me);
-    return reduce_part<P, XSG_F16, T, kEarly>(tab.base[t], part, me);
+    const int dtype = tab.entry[t].dtype;
+    if (dtype == XSG_F32) return reduce_part<P, XSG_F32, T, kEarly>(tab.entry[t].base, part, me);
+    if (dtype == XSG_BF16) return reduce_part<P, XSG_BF16, T, kEarly>(tab.entry[t].base, part, me);
+    return reduce_part<P, XSG_F16, T, kEarly>(tab.entry[t].base, part, me);
 }
 
 // Over the block, in a fixed order; every thread gets the result.  `smem`
@@ -423,10 +427,10 @@ __device__ __forceinline__ void scale_part(void* base, Part part, float c, int m
 
 template <int T, typename Table>
 __device__ __forceinline__ void scale_part(const Table& tab, int t, Part part, float c, int me) {
-    const int dtype = tab.dtype[t];
-    if (dtype == XSG_F32) scale_part<XSG_F32, T>(tab.base[t], part, c, me);
-    else if (dtype == XSG_BF16) scale_part<XSG_BF16, T>(tab.base[t], part, c, me);
-    else scale_part<XSG_F16, T>(tab.base[t], part, c, me);
+    const int dtype = tab.entry[t].dtype;
+    if (dtype == XSG_F32) scale_part<XSG_F32, T>(tab.entry[t].base, part, c, me);
+    else if (dtype == XSG_BF16) scale_part<XSG_BF16, T>(tab.entry[t].base, part, c, me);
+    else scale_part<XSG_F16, T>(tab.entry[t].base, part, c, me);
 }
 
 // The second pass of clipping.  c = 1 leaves the data alone.  The tiles are
@@ -1013,12 +1017,12 @@ struct SpanLaunch {
     int64_t first_span = 0, sums_at = 0, slots_at = 0, bytes = 0;
 
     void add(const void* data, int64_t n, int dtype) {
-        const int t = tab.count++;
+        SpanEntry& e = tab.entry[tab.count++];
         const auto at = reinterpret_cast<uintptr_t>(data);
-        tab.base[t] = reinterpret_cast<void*>(at - at % kLine);
-        tab.lead[t] = uint8_t(at % kLine / elem_size(dtype));
-        tab.end[t] = tab.lead[t] + n;
-        tab.dtype[t] = uint8_t(dtype);
+        e.base = reinterpret_cast<void*>(at - at % kLine);
+        e.lead = uint8_t(at % kLine / elem_size(dtype));
+        e.end = e.lead + n;
+        e.dtype = uint8_t(dtype);
         bytes += n * elem_size(dtype);
     }
     // The tiles, when all tensors are in.
@@ -1026,18 +1030,17 @@ struct SpanLaunch {
         tab.tile_bytes = tile_bytes;
         int64_t tiles = 0;
         for (int t = 0; t < tab.count; ++t) {
-            const int64_t per = tile_bytes / elem_size(tab.dtype[t]);
+            const SpanEntry& e = tab.entry[t];
+            const int64_t per = tile_bytes / elem_size(e.dtype);
             tab.first[t] = int32_t(tiles);
-            tiles += tab.end[t] > tab.lead[t] ? (tab.end[t] + per - 1) / per : 0;
+            tiles += e.end > e.lead ? (e.end + per - 1) / per : 0;
         }
         tab.first[tab.count] = int32_t(tiles);
         return int32_t(tiles);
     }
     void close(int64_t& sums, int64_t& slots) {
-        // from 16 KB on, larger tiles only where each block has many (clipping 118 M floats: 16 KB 238 us,
-        // 32 KB 236, 64 KB 240)
-        const bool many = bytes > (int64_t(32) << 10) * kOptBlocks * 8;
-        blocks = std::max(1, std::min(cut(many ? 32768 : tile_for(bytes, 4096, 16384, kOptBlocks)), kOptBlocks));
+        // clipping 90 M bf16 in 201 tensors: 73 us with tiles of 32 KB, 77 of 16; 118 M floats: 213, 217
+        blocks = std::max(1, std::min(cut(tile_for(bytes, 4096, 32768, kOptBlocks)), kOptBlocks));
         sums_at = sums;
         sums += blocks;
         slots_at = slots;
