@@ -21,8 +21,8 @@
 // Measured on B200, 6449 GB/s being a copy's rate: norm of 640 M floats
 // 351 us (7290 GB/s), of 160 M bf16 51 us (6220); clipping 118 M floats 213 us
 // (its three passes of 472 MB: 6650, of which the L2 serves some); the
-// clipped update of 118 M floats 571 us (3304 MB and the norm's 472: 6610), of
-// 150 M bf16 over masters 699 us (4.5 GB: 6440), of 35 % of 1 M rows of 59
+// clipped update of 118 M floats 567 us (3304 MB and the norm's 472: 6660), of
+// 150 M bf16 over masters 693 us (4.5 GB: 6490), of 35 % of 1 M rows of 59
 // floats 158 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
