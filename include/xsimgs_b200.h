@@ -565,7 +565,8 @@ int xsg_clip_grads(const xsg_span* spans_host, int64_t n_spans, int norm_type, f
                    void* workspace, size_t workspace_bytes, xsg_stream_t stream);
 /* One tensor of an AdamW update.  master (may be NULL): the 32-bit parameter
  * that `param` is a rounding of.  row_mask (may be NULL): n / row_size bytes,
- * rows of zero stay as they are (parameter and moments). */
+ * n a multiple of row_size; rows of zero stay as they are (parameter and
+ * moments). */
 typedef struct xsg_adamw_span {
     void* param;
     const void* grad;

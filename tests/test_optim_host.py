@@ -127,3 +127,17 @@ def test_optimizer_arguments():
     assert opt.param_groups[0]["lr"] == 0.5 and opt.param_groups[0]["betas"] == (0.8, 0.9)
     assert opt.step() is None  # no gradients: nothing to do
     assert "row_masks" in inspect.signature(opt.step).parameters
+
+
+def test_row_masks_cover_whole_rows(lib):
+    # a mask holds n / row_size bytes: elements past the last whole row would be looked up behind it
+    fake = 1 << 20
+
+    def adamw(n, row_size):
+        s = (AdamSpan * 1)(AdamSpan(param=fake, grad=fake, exp_avg=fake, exp_avg_sq=fake, row_mask=fake, n=n,
+                                    row_size=row_size, lr=0.1, beta1=0.9, beta2=0.99, eps=1e-8))
+        return lib.xsg_adamw_update(s, C.c_int64(1), C.c_void_p(fake), C.c_float(-1.0), 0, None, None, C.c_size_t(0),
+                                    None)
+
+    for n, row_size in ((10, 4), (3, 4), (1, 1 << 20), (1 << 20, 3)):
+        refuse(lib, adamw(n, row_size), 1, b"multiple of the row size")

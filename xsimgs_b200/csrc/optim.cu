@@ -1210,6 +1210,9 @@ int check_adamw(const xsg_adamw_span* spans, int64_t n) {
         XSG_REQUIRE(s.n == 0 || (s.param && s.grad && s.exp_avg && s.exp_avg_sq), "adamw_update: null pointer");
         XSG_REQUIRE(!s.row_mask || (s.row_size > 0 && s.row_size < (int64_t(1) << 30)),
                     "adamw_update: a row mask needs a row size below 2^30");
+        // the mask has n / row_size entries: elements past the last whole row have none
+        XSG_REQUIRE(!s.row_mask || s.n % s.row_size == 0,
+                    "adamw_update: the element count under a row mask must be a multiple of the row size");
         const auto off = [](const void* p, int size) { return reinterpret_cast<uintptr_t>(p) % size != 0; };
         XSG_REQUIRE(!off(s.param, elem_size(s.param_dtype)) && !off(s.grad, elem_size(s.grad_dtype)) &&
                         !off(s.exp_avg, 4) && !off(s.exp_avg_sq, 4) && !off(s.master, 4),
