@@ -548,7 +548,8 @@ typedef struct xsg_span {
     int32_t dtype; /* xsg_dtype */
 } xsg_span;
 /* Scratch of the three calls below: enough for any tensors, or for these
- * (0 where one launch does without). */
+ * (0 where one launch does without).  It is 8-byte aligned, as is `step`;
+ * norms are 4-byte aligned. */
 size_t xsg_grad_norm_workspace_size(int64_t n_spans);
 size_t xsg_grad_norm_workspace_bytes(const xsg_span* spans_host, int64_t n_spans);
 size_t xsg_clip_grads_workspace_bytes(const xsg_span* spans_host, int64_t n_spans);

@@ -141,3 +141,28 @@ def test_row_masks_cover_whole_rows(lib):
 
     for n, row_size in ((10, 4), (3, 4), (1, 1 << 20), (1 << 20, 3)):
         refuse(lib, adamw(n, row_size), 1, b"multiple of the row size")
+
+
+def test_words_of_a_call_are_aligned(lib):
+    # norms, the step counter and the scratch's 64-bit sums: an address between words is refused, not launched with
+    fake, size = 1 << 20, 1 << 20
+    spans = (Span * 1)(Span(fake, 1 << 22, 0))
+
+    def norm(out=fake, norms=None, ws=fake):
+        return lib.xsg_grad_norm(spans, C.c_int64(1), 2, C.c_void_p(out), C.c_void_p(norms), C.c_void_p(ws),
+                                 C.c_size_t(size), None)
+
+    def clip(out=fake, ws=fake):
+        return lib.xsg_clip_grads(spans, C.c_int64(1), 2, C.c_float(1.0), C.c_void_p(out), C.c_void_p(ws),
+                                  C.c_size_t(size), None)
+
+    def adamw(step=fake, out=fake, ws=fake, n=1 << 22):
+        s = (AdamSpan * 1)(AdamSpan(param=fake, grad=fake, exp_avg=fake, exp_avg_sq=fake, n=n, lr=0.1, beta1=0.9,
+                                    beta2=0.99, eps=1e-8))
+        return lib.xsg_adamw_update(s, C.c_int64(1), C.c_void_p(step), C.c_float(1.0), 0, C.c_void_p(out),
+                                    C.c_void_p(ws), C.c_size_t(size), None)
+
+    for rc in (lambda: norm(out=fake + 2), lambda: norm(norms=fake + 1), lambda: norm(ws=fake + 4),
+               lambda: clip(out=fake + 1), lambda: clip(ws=fake + 1), lambda: adamw(step=fake + 4),
+               lambda: adamw(out=fake + 3), lambda: adamw(ws=fake + 2), lambda: adamw(step=fake + 1, n=8)):
+        refuse(lib, rc(), 1, b"misaligned")

@@ -1009,6 +1009,17 @@ int check_spans(const xsg_span* spans, int64_t n, const char* what) {
     return XSG_OK;
 }
 
+// The words of a call that are no tensors: norms, the counter (64 bits), and
+// the scratch, which begins with sums in 64 bits.
+bool aligned(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+
+int check_words(const float* norm, const float* norms, const int64_t* step, const Arena& arena, const char* what) {
+    XSG_REQUIRE(aligned(norm, sizeof(float)) && aligned(norms, sizeof(float)), std::string(what) + ": misaligned norm");
+    XSG_REQUIRE(aligned(step, sizeof(int64_t)), std::string(what) + ": misaligned step counter");
+    XSG_REQUIRE(aligned(arena.base, sizeof(double)), std::string(what) + ": misaligned workspace");
+    return XSG_OK;
+}
+
 // The tensors of one launch.
 template <int N>
 struct SpanLaunch {
@@ -1171,6 +1182,7 @@ int grad_norm(const xsg_span* spans, int64_t n, int norm_type, float* norm, floa
               cudaStream_t st) {
     if (int rc = check_spans(spans, n, "grad_norm")) return rc;
     XSG_REQUIRE(norm, "grad_norm: null output");
+    if (int rc = check_words(norm, norms, nullptr, arena, "grad_norm")) return rc;
     if (arena.cap < xsg_grad_norm_workspace_bytes(spans, n))
         return set_error(XSG_ERR_WORKSPACE, "grad_norm: workspace too small");
     const auto get = [&](int64_t i, auto& L) { L.add(spans[i].data, spans[i].n, spans[i].dtype); };
@@ -1186,6 +1198,7 @@ int clip_grads(const xsg_span* spans, int64_t n, int norm_type, float max_norm, 
                cudaStream_t st) {
     if (int rc = check_spans(spans, n, "clip_grads")) return rc;
     XSG_REQUIRE(norm, "clip_grads: null output");
+    if (int rc = check_words(norm, nullptr, nullptr, arena, "clip_grads")) return rc;
     XSG_REQUIRE(max_norm >= 0.f && std::isfinite(max_norm), "clip_grads: max_norm must be finite and not negative");
     if (arena.cap < xsg_clip_grads_workspace_bytes(spans, n))
         return set_error(XSG_ERR_WORKSPACE, "clip_grads: workspace too small");
@@ -1321,6 +1334,7 @@ int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float ma
                  float* norm, Arena arena, cudaStream_t st) {
     if (int rc = check_adamw(spans, n)) return rc;
     XSG_REQUIRE(step, "adamw_update: null step counter");
+    if (int rc = check_words(norm, nullptr, step, arena, "adamw_update")) return rc;
     XSG_REQUIRE(max_norm < 0.f || std::isfinite(max_norm), "adamw_update: max_norm must be finite");
     ScopedTimer tm("adamw_update", st);
     AdamCall call{};
