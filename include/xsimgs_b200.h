@@ -583,8 +583,10 @@ typedef struct xsg_adamw_span {
 } xsg_adamw_span;
 size_t xsg_adamw_workspace_bytes(const xsg_adamw_span* spans_host, int64_t n_spans);
 /* step [2]: the number of updates taken so far, which the call advances by
- * one, and a word that has to be zero between calls (blocks fetch their tiles
- * from it; calls that share it follow one another).  With t = step + 1:
+ * one, and a word that has to be zero between calls (blocks count themselves
+ * in it).  Calls that share it follow one another: where they overlap, or the
+ * word is not zero, updates may be counted wrongly, and nothing else.  With
+ * t = step + 1:
  *   g' = c g, m <- b1 m + (1 - b1) g', v <- b2 v + (1 - b2) g'^2,
  *   w <- w - lr wd w - lr (m / (1 - b1^t)) / (sqrt(v / (1 - b2^t)) + eps).
  * max_norm >= 0: c is the clipping coefficient of all gradients' 2-norm (the

@@ -706,3 +706,64 @@ def test_instrumentation():
         ms, count = capi.timing_query(name)
         assert count == 1 and 0 < ms < 100
     capi.timing_reset()
+
+
+# --------------------------------------------- the counter's second word --
+def check_either_count(p, g, m, v, old, counts, lr, eps, c=1.0, masks=None):
+    """Every element updated once, with one of the counts' bias corrections."""
+    for i in range(len(p)):
+        found = torch.zeros(p[i].shape, dtype=torch.bool)
+        for t in counts:
+            (w1, m1, v1), (dw, dm, dv) = adamw64(*old[i], t, lr, (0.9, 0.999), eps, 0.0, c)
+            found |= ((p[i].double().cpu() - w1).abs() <= dw + HALF_ULP[torch.float32] * w1.abs() * 1.01)
+            near_m, near_v = (m[i].double().cpu() - m1).abs() <= dm, (v[i].double().cpu() - v1).abs() <= dv
+        moved = near_m & near_v & found
+        if masks is not None:
+            rows = masks[i].cpu().view([-1] + [1] * (p[i].dim() - 1)).expand(p[i].shape)
+            same = (p[i] == old[i][0]).cpu() & (m[i] == old[i][2]).cpu() & (v[i] == old[i][3]).cpu()
+            moved = torch.where(rows, moved, same)
+        assert moved.all()
+
+
+@pytest.mark.parametrize("word", [1, 3, 700, 1 << 20, -1])
+@pytest.mark.parametrize("kind", ["plain", "clip", "rows", "rows_clip"])
+@pytest.mark.parametrize("n", [3000, 300_000, 3_000_000])
+def test_adamw_updates_everything_whatever_the_second_word(word, kind, n):
+    # a counter whose second word was left wrong may cost an update's count, but no element its update
+    p, g, m, v, _ = state_for([3 * (n // 4), 3 * (n // 12) + 3], torch.float32, 17)
+    mask = None
+    if "rows" in kind:
+        p, g, m, v = ([x.view(-1, 3) for x in xs] for xs in (p, g, m, v))
+        mask = [torch.arange(x.shape[0], device="cuda") % 3 < 2 for x in p]
+    old = [tuple(x.clone() for x in q) for q in zip(p, g, m, v)]
+    norm = norm64(g, 2)
+    limit = 0.3 * norm if "clip" in kind else None
+    step = torch.tensor([4, word], dtype=torch.int64, device="cuda")
+    X.adamw_update_(p, g, m, v, step, lr=0.01, max_norm=limit, row_mask=mask)
+    check_either_count(p, g, m, v, old, (5, 6), 0.01, 1e-8, limit / (norm + CLIP_EPS) if limit else 1.0, mask)
+    if "clip" in kind:
+        assert int(step[0]) == 5
+
+
+@pytest.mark.parametrize("kind", ["plain", "clip", "rows"])
+def test_adamw_shared_counter_on_two_streams(kind):
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    step = X.adamw_step_counter("cuda", 4)
+    calls = []
+    for k in range(2):
+        p, g, m, v, _ = state_for([3 * 700_001 + 300_000 * k], torch.float32, 23 + k)
+        mask = None
+        if kind == "rows":
+            p, g, m, v = ([x.view(-1, 3) for x in xs] for xs in (p, g, m, v))
+            mask = [torch.arange(p[0].shape[0], device="cuda") % 3 < 2]
+        norm = norm64(g, 2)
+        calls.append((p, g, m, v, mask, 0.3 * norm if kind == "clip" else None,
+                      0.3 * norm / (norm + CLIP_EPS) if kind == "clip" else 1.0,
+                      [tuple(x.clone() for x in q) for q in zip(p, g, m, v)]))
+    torch.cuda.synchronize()
+    for s, (p, g, m, v, mask, limit, _, _) in zip(streams, calls):
+        with torch.cuda.stream(s):
+            X.adamw_update_(p, g, m, v, step, lr=0.01, max_norm=limit, row_mask=mask)
+    torch.cuda.synchronize()
+    for p, g, m, v, mask, _, c, old in calls:
+        check_either_count(p, g, m, v, old, (5, 6, 7), 0.01, 1e-8, c, mask)

@@ -14,7 +14,7 @@
 // tensor is cut into tiles.  Blocks (of small tensors, warps) take the tiles
 // of all tensors in turn where they are summed, so that the order of every sum
 // depends on the tensors' sizes and offsets alone: the same bits on every run.
-// Where they are written, blocks fetch them from a counter.  A second pass is
+// Where a second pass writes them, blocks fetch them from a counter; it is
 // launched while the first one ends and starts at the tiles that the first one
 // read last.
 //
@@ -23,7 +23,7 @@
 // (its three passes of 472 MB: 6650, of which the L2 serves some); the
 // clipped update of 118 M floats 567 us (3304 MB and the norm's 472: 6660), of
 // 150 M bf16 over masters 693 us (4.5 GB: 6490), of 35 % of 1 M rows of 59
-// floats 158 us.
+// floats 159 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -91,6 +91,8 @@ struct SpanTable {
     int32_t first[N + 1];
     int32_t count;
     int32_t tile_bytes;
+    int32_t counters;  // of the launches of a second pass, which this one zeroes (as a
+                       // parameter of its own the number costs the host 0.3 us a launch)
 };
 
 // The part of tensor t in the tiles [tile, stop): numbers [lo, hi).
@@ -293,7 +295,8 @@ __global__ void __launch_bounds__(kOptThreads, kNormResident)
                         unsigned* __restrict__ fetched) {
     __shared__ double smem[33];
     pdl_trigger();
-    if (fetched && blockIdx.x == 0 && threadIdx.x == 0) *fetched = 0;  // for the second pass
+    if (fetched && blockIdx.x == 0)  // the tile counters of the second pass
+        for (int i = threadIdx.x; i < tab.counters; i += blockDim.x) fetched[i] = 0;
     const int32_t tiles = tab.first[tab.count];
     double acc = 0.0;
     int t = -1;
@@ -639,7 +642,8 @@ struct AdamTable {
 };
 
 struct AdamCall {
-    unsigned long long* step;  // [0] updates taken, [1] tiles fetched (zero between launches)
+    unsigned long long* step;  // [0] updates taken, [1] blocks that are done, modulo the launch's
+    unsigned* fetched;         // tiles fetched (behind a norm, which zeroes it)
     const double* sums;        // the gradients' partial sums, or null
     int32_t n_sums;
     int32_t advance;      // the call's last launch counts the update
@@ -871,15 +875,22 @@ __device__ __forceinline__ void adam_tile(const Table& tab, int t, int32_t tile,
     adam_part<kF32, kRows, T>(e, {max(int64_t(e.lead), at), min(e.end, at + tab.tile)}, h, me);
 }
 
-// Blocks fetch tiles as in clipping, from the last to the first.  Every block
-// fetches one past the last; the last of them to do so leaves the counter at
-// zero and counts the update, when all blocks that have had a tile have long
-// read step[0].
+// Behind a norm, blocks fetch tiles as in clipping, from the last to the first.
+// Every block fetches one past the last; the last of them to do so counts the
+// update, when all blocks that have had a tile have long read step[0].  The
+// counter is in the call's scratch, where the norm's pass zeroes it.  A call
+// without a norm has no scratch and nothing in the L2 to meet: a block for each
+// tile (118 M floats: 495 us, 494 with a counter; 1.4 M floats:
+// 8.2 us, 11.2), under row masks, which cost more to set out on, 740 blocks that
+// take tiles in turn (1 M rows, 35 % seen: 158.7 us, 157.8 with a counter; 200 k
+// rows: 41.5, 42.0).  There the last block to be done counts the update, by
+// step[1] modulo the number of blocks: if that word is not zero, blocks count
+// too early, but each tile is still updated once.
 template <int N, bool kF32, bool kRows>
 __global__ void __launch_bounds__(kOptThreads, kAdamResident)
     adamw_kernel(const __grid_constant__ AdamTable<N> tab, const __grid_constant__ AdamCall call) {
     __shared__ double smem[33];
-    __shared__ uint64_t next[2];
+    __shared__ uint32_t next[2];
     AdamScale h;
     h.c = 1.f;
     if (call.sums) {
@@ -891,12 +902,15 @@ __global__ void __launch_bounds__(kOptThreads, kAdamResident)
     }
     const float steps = float(call.step[0] + 1);
     const uint32_t tiles = uint32_t(tab.first[tab.count]);
-    if (threadIdx.x == 0) next[0] = atomicAdd(call.step + 1, 1ull);
+    const auto fetch = [&](uint32_t before) {
+        return call.fetched ? atomicAdd(call.fetched, 1u) : before + gridDim.x;
+    };
+    if (threadIdx.x == 0) next[0] = call.fetched ? fetch(0) : blockIdx.x;
     __syncthreads();
     int t = -1, turn = 0;
     for (; next[turn] < tiles; turn ^= 1) {
-        const int32_t tile = int32_t(tiles - 1u - uint32_t(next[turn]));
-        if (threadIdx.x == 0) next[turn ^ 1] = atomicAdd(call.step + 1, 1ull);
+        const int32_t tile = int32_t(tiles - 1u - next[turn]);
+        if (threadIdx.x == 0) next[turn ^ 1] = fetch(next[turn]);
         if (t < 0 || tile < tab.first[t]) {
             if (t < 0) t = owner_of(tab, tile);
             while (tile < tab.first[t]) --t;
@@ -905,9 +919,11 @@ __global__ void __launch_bounds__(kOptThreads, kAdamResident)
         adam_tile<kF32, kRows, kOptThreads>(tab, t, tile, h, threadIdx.x);
         __syncthreads();
     }
-    if (threadIdx.x == 0 && next[turn] == uint64_t(tiles) + gridDim.x - 1) {
-        if (call.advance) call.step[0] += 1;
-        call.step[1] = 0;
+    if (threadIdx.x == 0 && call.advance) {
+        const bool last = call.fetched ? next[turn] == tiles + gridDim.x - 1u
+                                       : atomicInc(reinterpret_cast<unsigned*>(call.step + 1), gridDim.x - 1u) ==
+                                             gridDim.x - 1u;
+        if (last) atomicAdd(call.step, 1ull);
     }
 }
 
@@ -932,7 +948,7 @@ __global__ void __launch_bounds__(kSmallThreads)
         group_of = t;
         adam_tile<kF32, true, 32>(tab, t, tile, h, w.lane);
     });
-    if (first) call.step[0] += 1;  // all have read it before the norm's barriers
+    if (first) atomicAdd(call.step, 1ull);  // all have read it before the norm's barriers
 }
 
 // ------------------------------------------------------------------ host --
@@ -1057,11 +1073,16 @@ struct SpanLaunch {
         slots_at = slots;
         slots += blocks + tab.count;
     }
-    SpanLaunch() { tab.count = 0; }
+    SpanLaunch() { tab.count = tab.counters = 0; }
 };
 
 size_t sums_count(int64_t n_spans) { return size_t((n_spans + kSpans - 1) / kSpans) * kOptBlocks; }
 size_t slots_count(int64_t n_spans) { return sums_count(n_spans) + size_t(n_spans); }
+
+// Tile counters, one for each launch of a second pass: an update's takes
+// kAdamGroups tensors at least unless it is the last, clipping's more.
+static_assert(kAdamGroups <= kSmallSpans && kAdamGroups <= kSpans && kAdamGroups <= kAdamSpans, "counters_count");
+int64_t counters_count(int64_t n_spans) { return n_spans / kAdamGroups + 1; }
 
 // All launches over `n` tensors, tensor i from get(i): one of a small table
 // where that holds them, else as many of the large table as it takes.
@@ -1078,6 +1099,7 @@ struct SpanPlan {
             get(i, L);
         }
         for (auto& L : launches) L.close(sums, slots);
+        launches[0].tab.counters = int32_t(counters_count(n));
     }
 
     int64_t bytes() const { return launches[0].bytes; }
@@ -1091,7 +1113,7 @@ struct SpanPlan {
                              sums_at + L.sums_at, slots_at + L.slots_at);
             else
                 launch_table(norm_partial_kernel<P, N>, L.blocks, kOptThreads, 1, false, st, L.tab,
-                             sums_at + L.sums_at, fetched ? fetched + l : nullptr);
+                             sums_at + L.sums_at, fetched);
         }
     }
 };
@@ -1152,7 +1174,7 @@ int clip_all(const SpanPlan<N>& plan, float max_norm, float* norm, Arena arena, 
         }
     }
     double* sums = arena.take<double>(sums_count(n));
-    unsigned* fetched = arena.take<unsigned>(plan.launches.size());
+    unsigned* fetched = arena.take<unsigned>(counters_count(n));
     plan.template partials<P>(sums, nullptr, fetched, st);
     for (size_t l = plan.launches.size(); l-- > 0;)
         launch_table(clip_scale_kernel<P, N>, std::min(plan.launches[l].blocks, 148 * kScaleResident), kOptThreads, 1, l + 1 == plan.launches.size(),
@@ -1322,11 +1344,13 @@ void adamw_all(const xsg_adamw_span* spans, int64_t n, int64_t elems, AdamCall c
         i = fill_adam(tab, spans, i, n, tile, f32, rows);
         call.advance = i >= n;
         call.norm = i >= n ? norm : nullptr;
-        const int blocks = std::max(1, std::min(tab.first[tab.count], 148 * kAdamResident));
+        const int32_t tiles = tab.first[tab.count];
+        const int32_t blocks = std::max(1, call.fetched || rows ? std::min(tiles, 148 * kAdamResident) : tiles);
         launch_table(f32 ? (rows ? adamw_kernel<N, true, true> : adamw_kernel<N, true, false>)
                          : (rows ? adamw_kernel<N, false, true> : adamw_kernel<N, false, false>),
                      blocks, kOptThreads, 1, pdl, st, tab, call);
         pdl = false;
+        if (call.fetched) ++call.fetched;
     }
 }
 
@@ -1365,7 +1389,8 @@ int adamw_update(const xsg_adamw_span* spans, int64_t n, int64_t* step, float ma
                 }
             }
             double* sums = arena.take<double>(sums_count(n));
-            plan.template partials<2>(sums, nullptr, nullptr, st);
+            call.fetched = arena.take<unsigned>(counters_count(n));
+            plan.template partials<2>(sums, nullptr, call.fetched, st);
             call.sums = sums;
             call.n_sums = int(plan.sums);
             return int(XSG_OK);

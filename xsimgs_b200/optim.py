@@ -49,8 +49,9 @@ def clip_gradients_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: f
 def adamw_step_counter(device, updates: int = 0) -> torch.Tensor:
     """The `step` of `adamw_update_`: the number of updates taken, which the
     call advances on the device, and a word that has to be zero between calls
-    (the call's blocks fetch their tiles from it), so that calls that share a
-    counter follow one another on a stream."""
+    (the call's blocks count themselves in it), so that calls that share a
+    counter follow one another on a stream.  Where they do not, updates may be
+    counted wrongly; every element is still updated once by each."""
     return torch.tensor([updates, 0], dtype=torch.int64, device=device)
 
 
