@@ -767,3 +767,27 @@ def test_adamw_shared_counter_on_two_streams(kind):
     torch.cuda.synchronize()
     for p, g, m, v, mask, _, c, old in calls:
         check_either_count(p, g, m, v, old, (5, 6, 7), 0.01, 1e-8, c, mask)
+
+
+# ------------------------------------------- checkpoints of stock optimisers --
+def test_optimizer_goes_on_from_a_stock_checkpoint():
+    def grads(ps, k):
+        for p in ps:
+            p.grad = (1 + k) * p.detach().sin()
+
+    torch.manual_seed(5)
+    a = [torch.randn(300, 3, device="cuda", requires_grad=True), torch.randn(41, device="cuda", requires_grad=True)]
+    theirs = torch.optim.AdamW(a, lr=3e-3, weight_decay=0.1)
+    for k in range(4):
+        grads(a, k)
+        theirs.step()
+    b = [p.detach().clone().requires_grad_() for p in a]
+    ours = X.AdamW(b)
+    ours.load_state_dict(theirs.state_dict())
+    for k in range(4):
+        for ps, opt in ((a, theirs), (b, ours)):
+            grads(ps, k)
+            opt.step()
+        for x, y in zip(a, b):
+            assert (x - y).abs().max() <= 1e-6 * (1 + k)
+    assert ours._step.tolist() == [8, 0]

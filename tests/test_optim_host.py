@@ -166,3 +166,49 @@ def test_words_of_a_call_are_aligned(lib):
                lambda: clip(out=fake + 1), lambda: clip(ws=fake + 1), lambda: adamw(step=fake + 4),
                lambda: adamw(out=fake + 3), lambda: adamw(ws=fake + 2), lambda: adamw(step=fake + 1, n=8)):
         refuse(lib, rc(), 1, b"misaligned")
+
+
+def stock_checkpoint(updates=50, dtype=torch.float32):
+    # what torch.optim.AdamW leaves behind: an update count with each parameter, none for all
+    torch.manual_seed(1)
+    ps = [torch.randn(7, 3, dtype=dtype, requires_grad=True), torch.randn(5, dtype=dtype, requires_grad=True)]
+    opt = torch.optim.AdamW(ps, lr=1e-2)
+    for _ in range(updates):
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        opt.step()
+    return ps, opt.state_dict()
+
+
+def test_optimizer_takes_the_count_of_a_stock_checkpoint():
+    import xsimgs_b200 as X
+    ps, saved = stock_checkpoint()
+    opt = X.AdamW(ps)
+    opt.load_state_dict(saved)
+    assert opt._step.tolist() == [50, 0]
+    for i, p in enumerate(ps):
+        assert set(opt.state[p]) == {"exp_avg", "exp_avg_sq"}
+        for k in opt.state[p]:
+            assert torch.equal(opt.state[p][k], saved["state"][i][k])
+    again = opt.state_dict()
+    assert again["updates"] == 50
+    # the count survives what keeps state and groups alone, as sharded and converted checkpoints do
+    other = X.AdamW(ps)
+    other.load_state_dict({k: again[k] for k in ("state", "param_groups")})
+    assert other._step.tolist() == [50, 0]
+    fresh = X.AdamW(ps)
+    fresh.load_state_dict({k: v for k, v in X.AdamW(ps).state_dict().items() if k != "updates"})
+    assert fresh._step.tolist() == [0, 0]
+
+
+def test_optimizer_refuses_moments_without_one_count():
+    import xsimgs_b200 as X
+    ps, saved = stock_checkpoint(3)
+    differ = {**saved, "state": {i: {**s, "step": s["step"] + i} for i, s in saved["state"].items()}}
+    missing = {**saved, "state": {i: {k: v for k, v in s.items() if k != "step" or i} for i, s in
+                                  saved["state"].items()}}
+    for bad in (differ, missing):
+        opt = X.AdamW(ps, lr=0.25)
+        with pytest.raises(ValueError, match="updates"):
+            opt.load_state_dict(bad)
+        assert not opt.state and opt._step is None and opt.param_groups[0]["lr"] == 0.25  # as it was

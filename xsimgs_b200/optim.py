@@ -84,6 +84,18 @@ def adamw_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                             max_norm, skip_nonfinite, masters, row_mask)
 
 
+def _updates_of(state_dict: dict) -> int:
+    """The number of updates behind a checkpoint's moments."""
+    if "updates" in state_dict:
+        return int(state_dict["updates"])
+    counts = {int(s["step"]) if "step" in s else None for s in state_dict["state"].values() if s}
+    if not counts:
+        return 0
+    if len(counts) > 1 or None in counts:
+        raise ValueError("AdamW: the checkpoint has no number of updates that holds for all its parameters")
+    return counts.pop()
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW over `adamw_update_`: all parameter groups in one update.
 
@@ -152,17 +164,24 @@ class AdamW(torch.optim.Optimizer):
                 "_step": self._step}
 
     def state_dict(self) -> dict:
+        """The count of updates is in it once for all (`updates`) and, for what
+        keeps state and groups alone, with each parameter (`step`)."""
         d = super().state_dict()
         d["updates"] = 0 if self._step is None else int(self._step[0])
+        d["state"] = {i: {**s, "step": torch.tensor(float(d["updates"]))} for i, s in d["state"].items()
+                      if s}
         return d
 
     def load_state_dict(self, state_dict: dict) -> None:
+        """Takes `state_dict` of this class, or of `torch.optim.AdamW` if all
+        its parameters have had the same number of updates."""
+        updates = _updates_of(state_dict)
         super().load_state_dict({k: v for k, v in state_dict.items() if k != "updates"})
         # the base class casts state to its parameter's type: masters and moments stay in 32 bits
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, mine):
-            for k, v in state_dict["state"].get(i, {}).items():
-                self.state[p][k] = v.to(device=p.device, dtype=torch.float32, copy=True)
-        device = mine[0].device
-        self._step = adamw_step_counter(device, int(state_dict.get("updates", 0)))
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.to(device=p.device, dtype=torch.float32, copy=True)
+                                 for k, v in state_dict["state"][i].items() if k != "step"}
+        self._step = adamw_step_counter(mine[0].device, updates)
