@@ -791,3 +791,20 @@ def test_optimizer_goes_on_from_a_stock_checkpoint():
         for x, y in zip(a, b):
             assert (x - y).abs().max() <= 1e-6 * (1 + k)
     assert ours._step.tolist() == [8, 0]
+
+
+def test_optimizer_gives_loaded_half_parameters_masters():
+    p = torch.randn(1000, device="cuda").to(torch.bfloat16).requires_grad_()
+    stock = torch.optim.AdamW([p], lr=1e-3)
+    p.grad = torch.ones_like(p)
+    stock.step()
+    ours = X.AdamW([p])
+    ours.load_state_dict(stock.state_dict())
+    before = p.detach().float()
+    for k in range(40):  # steps of 1e-5, below the parameter's spacing for most: only masters keep them
+        for g in ours.param_groups:
+            g["lr"], g["weight_decay"] = 1e-5, 0.0
+        ours.step()
+    master = ours.state[p]["master"]
+    assert torch.equal(p.detach(), master.to(torch.bfloat16)) and ours._step.tolist() == [41, 0]
+    assert ((before - master) > 3e-4).all()  # 40 steps of 1e-5 against gradients of one

@@ -212,3 +212,22 @@ def test_optimizer_refuses_moments_without_one_count():
         with pytest.raises(ValueError, match="updates"):
             opt.load_state_dict(bad)
         assert not opt.state and opt._step is None and opt.param_groups[0]["lr"] == 0.25  # as it was
+
+
+def test_optimizer_completes_a_loaded_state():
+    # moments of 32-bit or stock training on half-precision parameters: the missing master comes from the parameter
+    import xsimgs_b200 as X
+    ps, saved = stock_checkpoint(3, torch.bfloat16)
+    opt = X.AdamW(ps)
+    opt.load_state_dict(saved)
+    for i, p in enumerate(ps):
+        s = opt._state(p)
+        assert s["master"].dtype == torch.float32 and torch.equal(s["master"], p.detach().float())
+        assert torch.equal(s["exp_avg"], saved["state"][i]["exp_avg"].float())
+        kept = s["master"]
+        assert opt._state(p)["master"] is kept
+    p = torch.zeros(3, requires_grad=True)
+    opt = X.AdamW([p])
+    opt.state[p]["exp_avg"] = torch.ones(3)
+    s = opt._state(p)
+    assert torch.equal(s["exp_avg"], torch.ones(3)) and torch.equal(s["exp_avg_sq"], torch.zeros(3)) and len(s) == 2

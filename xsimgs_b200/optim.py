@@ -115,12 +115,12 @@ class AdamW(torch.optim.Optimizer):
         self._step: torch.Tensor | None = None
 
     def _state(self, p: torch.Tensor) -> dict:
-        s = self.state[p]
-        if not s:
-            s["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
-            s["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
-            if p.dtype != torch.float32:
-                s["master"] = p.detach().to(torch.float32, copy=True)
+        s = self.state[p]  # what a checkpoint has left out begins here
+        for k in ("exp_avg", "exp_avg_sq"):
+            if k not in s:
+                s[k] = torch.zeros_like(p, dtype=torch.float32)
+        if p.dtype != torch.float32 and "master" not in s:
+            s["master"] = p.detach().to(torch.float32, copy=True)
         return s
 
     @torch.no_grad()
