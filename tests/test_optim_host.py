@@ -231,3 +231,22 @@ def test_optimizer_completes_a_loaded_state():
     opt.state[p]["exp_avg"] = torch.ones(3)
     s = opt._state(p)
     assert torch.equal(s["exp_avg"], torch.ones(3)) and torch.equal(s["exp_avg_sq"], torch.zeros(3)) and len(s) == 2
+
+
+def test_optimizer_refuses_checkpoints_of_other_rules():
+    import xsimgs_b200 as X
+    ps, _ = stock_checkpoint(1)
+    for cls, kw, match in ((torch.optim.AdamW, dict(amsgrad=True), "amsgrad"),
+                           (torch.optim.AdamW, dict(maximize=True), "maximize"),
+                           (torch.optim.Adam, dict(weight_decay=0.1), "decay")):
+        stock = cls(ps, **kw)
+        stock.step()
+        opt = X.AdamW(ps)
+        with pytest.raises(ValueError, match=match):
+            opt.load_state_dict(stock.state_dict())
+        assert not opt.state and opt._step is None
+    stock = torch.optim.Adam(ps)  # without decay the rules are the same
+    stock.step()
+    opt = X.AdamW(ps)
+    opt.load_state_dict(stock.state_dict())
+    assert opt._step.tolist() == [1, 0]

@@ -173,9 +173,16 @@ class AdamW(torch.optim.Optimizer):
         return d
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """Takes `state_dict` of this class, or of `torch.optim.AdamW` if all
-        its parameters have had the same number of updates."""
+        """Takes `state_dict` of this class, or of `torch.optim.AdamW` (and
+        `torch.optim.Adam` without decay) if all its parameters have had the
+        same number of updates, without `amsgrad` and `maximize`."""
         updates = _updates_of(state_dict)
+        for group in state_dict["param_groups"]:
+            for option in ("amsgrad", "maximize"):
+                if group.get(option):
+                    raise ValueError(f"AdamW: {option} is not supported")
+            if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
+                raise ValueError("AdamW: the checkpoint's weight decay goes through its gradients")
         super().load_state_dict({k: v for k, v in state_dict.items() if k != "updates"})
         # the base class casts state to its parameter's type: masters and moments stay in 32 bits
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
