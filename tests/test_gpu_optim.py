@@ -808,3 +808,24 @@ def test_optimizer_gives_loaded_half_parameters_masters():
     master = ours.state[p]["master"]
     assert torch.equal(p.detach(), master.to(torch.bfloat16)) and ours._step.tolist() == [41, 0]
     assert ((before - master) > 3e-4).all()  # 40 steps of 1e-5 against gradients of one
+
+
+def test_optimizer_closure():
+    p = torch.full((300,), 2.0, device="cuda", requires_grad=True)
+    q = p.detach().clone().requires_grad_()
+    opt, other = X.AdamW([p], lr=0.1, max_norm=1.0), X.AdamW([q], lr=0.1, max_norm=1.0)
+
+    def closure():
+        opt.zero_grad()
+        loss = p.square().sum()
+        loss.backward()
+        return loss
+
+    loss = opt.step(closure)
+    assert float(loss) == 1200.0
+    q.grad = 2.0 * q.detach()
+    norm = other.step()
+    assert torch.equal(opt.grad_norm, norm) and other.grad_norm is norm
+    assert torch.equal(p, q)
+    plain = X.AdamW([q], lr=0.1)
+    assert plain.step() is None and plain.grad_norm is None

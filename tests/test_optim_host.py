@@ -250,3 +250,11 @@ def test_optimizer_refuses_checkpoints_of_other_rules():
     opt = X.AdamW(ps)
     opt.load_state_dict(stock.state_dict())
     assert opt._step.tolist() == [1, 0]
+
+
+def test_optimizer_step_returns_the_closure_s_loss():
+    import xsimgs_b200 as X
+    p = torch.zeros(3, requires_grad=True)
+    opt = X.AdamW([p], max_norm=1.0)
+    assert opt.step(lambda: 2.5) == 2.5 and opt.grad_norm is None  # no gradients: no update, no norm
+    assert opt.step() is None

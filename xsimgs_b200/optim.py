@@ -103,7 +103,10 @@ class AdamW(torch.optim.Optimizer):
     2-norm over all groups; `skip_nonfinite` passes over steps whose norm is
     NaN or infinite.  Half-precision parameters get float32 masters.  The
     number of updates is one counter on the device for all parameters, so a
-    parameter added later starts at the common count."""
+    parameter added later starts at the common count.  `grad_norm`: the norm
+    before clipping of the last `step`, on the device."""
+
+    grad_norm: torch.Tensor | None = None
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
                  *, max_norm: float | None = None, skip_nonfinite: bool = False):
@@ -124,14 +127,20 @@ class AdamW(torch.optim.Optimizer):
         return s
 
     @torch.no_grad()
-    def step(self, closure=None, *, row_masks: dict | None = None) -> torch.Tensor | None:
+    def step(self, closure=None, *, row_masks: dict | None = None):
         """Updates every parameter that has a gradient; returns the global
         gradient norm before clipping (None without `max_norm` and
-        `skip_nonfinite`).  `row_masks`: for a parameter, the rows to
+        `skip_nonfinite`) or, given a `closure`, what that returns (the norm is
+        in `grad_norm` either way).  `row_masks`: for a parameter, the rows to
         update; the others keep their values and moments."""
+        loss = None
         if closure is not None:
             with torch.enable_grad():
-                closure()
+                loss = closure()
+        self.grad_norm = self._update(row_masks)
+        return self.grad_norm if closure is None else loss
+
+    def _update(self, row_masks: dict | None) -> torch.Tensor | None:
         params, grads, ms, vs, masters, masks = [], [], [], [], [], []
         lr, b1, b2, eps, decay = [], [], [], [], []
         for group in self.param_groups:
