@@ -829,3 +829,15 @@ def test_optimizer_closure():
     assert torch.equal(p, q)
     plain = X.AdamW([q], lr=0.1)
     assert plain.step() is None and plain.grad_norm is None
+
+
+def test_norms_hold_their_own_words_only():
+    # a kept or saved norm must not keep or save the scratch of its call
+    p, g, m, v, _ = state_for([700_000, 5], torch.float32, 5)
+    step = X.adamw_step_counter("cuda")
+    total, each = X.gradient_norm(g, per_tensor=True)
+    norms = [X.gradient_norm(g), total, X.clip_gradients_(g, 1e-3),
+             X.adamw_update_(p, g, m, v, step, lr=0.1, max_norm=1.0),
+             X.adamw_update_(p, g, m, v, step, lr=0.1, skip_nonfinite=True)]
+    assert all(n.shape == () and n.untyped_storage().nbytes() == 4 for n in norms)
+    assert each.untyped_storage().nbytes() == 8

@@ -4,7 +4,9 @@
 // layouts and error wording.  Each op checks its tensors, allocates outputs
 // and scratch with the caching allocator and calls the C ABI of
 // libxsimgs_b200.so (include/xsimgs_b200.h) on the current CUDA stream.
+#include <ATen/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -1033,25 +1035,21 @@ int norm_code(double p) {
     return XSG_NORM_INF;
 }
 
-// A norm and the scratch behind it in one allocation; the norm is a 0-dim
-// tensor on its first word (a second allocation costs a microsecond, a tenth
-// of a call over small tensors).
+// A norm and the scratch of its call, on the current device.  The norm is a
+// tensor of its own: a caller may keep it or save it.  The scratch needs no
+// tensor around it, and neither of them the dispatcher (together half a
+// microsecond, a twentieth of a call over small tensors).
 struct NormOutput {
-    Tensor buffer, norm;
+    Tensor norm;
+    c10::DataPtr buffer;
     size_t bytes;
-    NormOutput(size_t scratch, const Tensor& like) : bytes(scratch) {
-        const auto f32 = like.options().dtype(at::kFloat).requires_grad(false);
-        if (!bytes) {
-            norm = at::empty({}, f32);
-            return;
-        }
-        buffer = at::empty({int64_t(kWords + (bytes + 3) / 4)}, f32);
-        norm = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buffer.storage()),
-                                                        buffer.key_set(), buffer.dtype());
-        norm.unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef{}, c10::IntArrayRef{});
+    explicit NormOutput(size_t scratch) : bytes(scratch) {
+        c10::Allocator* memory = c10::cuda::CUDACachingAllocator::get();
+        norm = at::detail::empty_generic({}, memory, c10::DispatchKeySet(c10::DispatchKey::CUDA), at::kFloat,
+                                         std::nullopt);
+        if (bytes) buffer = memory->allocate(bytes);
     }
-    void* scratch() const { return bytes ? fptr_mut(buffer) + kWords : nullptr; }
-    static constexpr int kWords = 64;  // keeps the scratch on a 256-byte boundary
+    void* scratch() const { return buffer.get(); }
 };
 
 py::object gradient_norm(const py::object& grads_seq, double norm_type, bool per_tensor) {
@@ -1071,7 +1069,7 @@ py::object gradient_norm(const py::object& grads_seq, double norm_type, bool per
         spans[i] = {t.data_ptr(), t.numel(), dtype};
     }
     const auto f32 = grads[0].options().dtype(at::kFloat).requires_grad(false);
-    const NormOutput out(xsg_grad_norm_workspace_bytes(spans.data(), int64_t(spans.size())), grads[0]);
+    const NormOutput out(xsg_grad_norm_workspace_bytes(spans.data(), int64_t(spans.size())));
     Tensor norms = per_tensor ? at::empty({int64_t(grads.size())}, f32) : Tensor();
     check(xsg_grad_norm(spans.data(), int64_t(spans.size()), p, fptr_mut(out.norm),
                         per_tensor ? fptr_mut(norms) : nullptr, out.scratch(), out.bytes, stream()));
@@ -1095,7 +1093,7 @@ Tensor clip_gradients(const py::object& grads_seq, double max_norm, double norm_
     }
     check_apart(extents, "clip_gradients_");
     c10::cuda::CUDAGuard g(grads[0].device());
-    const NormOutput out(xsg_clip_grads_workspace_bytes(spans.data(), int64_t(spans.size())), grads[0]);
+    const NormOutput out(xsg_clip_grads_workspace_bytes(spans.data(), int64_t(spans.size())));
     for (size_t i = 0; i < grads.size(); ++i) torch::autograd::impl::bump_version(grads[i]);
     check(xsg_clip_grads(spans.data(), int64_t(spans.size()), p, float(max_norm), fptr_mut(out.norm), out.scratch(),
                          out.bytes, stream()));
@@ -1191,7 +1189,7 @@ std::optional<Tensor> adamw_update(const py::object& params_seq, const py::objec
     check_apart(extents, "adamw_update_");
     const bool normed = max_norm.has_value() || skip_nonfinite;
     std::optional<NormOutput> out;
-    if (normed) out.emplace(xsg_adamw_workspace_bytes(spans.data(), int64_t(n)), params[0]);
+    if (normed) out.emplace(xsg_adamw_workspace_bytes(spans.data(), int64_t(n)));
     for (size_t i = 0; i < n; ++i) {
         torch::autograd::impl::bump_version(params[i]);
         torch::autograd::impl::bump_version(exp_avgs[i]);
