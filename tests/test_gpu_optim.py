@@ -841,3 +841,18 @@ def test_norms_hold_their_own_words_only():
              X.adamw_update_(p, g, m, v, step, lr=0.1, skip_nonfinite=True)]
     assert all(n.shape == () and n.untyped_storage().nbytes() == 4 for n in norms)
     assert each.untyped_storage().nbytes() == 8
+
+
+def test_operators_stand_outside_autograd():
+    # gradients with a graph of their own (create_graph): values are taken, no graph is built, and the documents say so
+    x = torch.randn(3000, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(x.pow(3).sum(), x, create_graph=True)
+    assert g.requires_grad
+    total, each = X.gradient_norm([g], per_tensor=True)
+    assert not total.requires_grad and not each.requires_grad
+    h = g * 1.0
+    assert not X.clip_gradients_([h], 1.0).requires_grad
+    p, m, v = x.detach().clone().requires_grad_(), torch.zeros(3000, device="cuda"), torch.zeros(3000, device="cuda")
+    assert not X.adamw_update_([p], [g], [m], [v], X.adamw_step_counter("cuda"), lr=0.1, max_norm=1.0).requires_grad
+    for f in (X.gradient_norm, X.clip_gradients_, X.adamw_update_):
+        assert "outside autograd" in " ".join(f.__doc__.split())

@@ -34,15 +34,18 @@ def gradient_norm(grads: Sequence[torch.Tensor], norm_type: float = 2.0, per_ten
     with each one's norm.  Sums are held in 64 bits, so large and tiny
     gradients neither overflow nor vanish on the way; NaN and infinite
     elements show in the result.  A tensor with gaps or expanded dimensions is
-    copied first."""
+    copied first.  The norm is taken outside autograd: nothing flows back
+    through it, whether or not the gradients have a graph (`create_graph`)."""
     return _C.gradient_norm(grads, norm_type, per_tensor)
 
 
 def clip_gradients_(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
     """Multiplies `grads` in place by min(1, max_norm / (norm + 1e-6)) and
     returns the norm that they had.  An infinite norm gives the factor 0, a
-    NaN makes every gradient NaN.  The tensors must be dense and may not share
-    memory."""
+    NaN makes every gradient NaN.  The scaling is outside autograd: a graph
+    that the gradients have knows nothing of it.  The tensors must be dense and
+    may not share memory.  For the norm alone, without a limit, there is
+    `gradient_norm`."""
     return _C.clip_gradients_(grads, max_norm, norm_type)
 
 
