@@ -258,3 +258,13 @@ def test_optimizer_step_returns_the_closure_s_loss():
     opt = X.AdamW([p], max_norm=1.0)
     assert opt.step(lambda: 2.5) == 2.5 and opt.grad_norm is None  # no gradients: no update, no norm
     assert opt.step() is None
+
+
+def test_options_fit_32_bits(lib):
+    # finite in 64 bits, infinite in the 32 of the update: inf * 0 would make NaN of untouched parameters
+    fake = 1 << 20
+    for kw in (dict(lr=1e39), dict(lr=-1e39), dict(lr=1e20, weight_decay=1e20), dict(lr=1e-3, weight_decay=1e308)):
+        f = dict(param=fake, grad=fake, exp_avg=fake, exp_avg_sq=fake, n=8, beta1=0.9, beta2=0.99, eps=1e-8)
+        s = (AdamSpan * 1)(AdamSpan(**{**f, **kw}))
+        refuse(lib, lib.xsg_adamw_update(s, C.c_int64(1), C.c_void_p(fake), C.c_float(-1.0), 0, None, None,
+                                         C.c_size_t(0), None), 1, b"learning rate")

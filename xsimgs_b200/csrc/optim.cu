@@ -1255,6 +1255,9 @@ int check_adamw(const xsg_adamw_span* spans, int64_t n) {
         XSG_REQUIRE(s.beta1 >= 0 && s.beta1 < 1 && s.beta2 >= 0 && s.beta2 < 1, "adamw_update: betas must be in [0, 1)");
         XSG_REQUIRE(s.eps >= 0 && std::isfinite(s.lr) && std::isfinite(s.weight_decay),
                     "adamw_update: bad learning rate, eps or weight decay");
+        // finite in 64 bits is not enough: inf * 0 would make NaN of entries without gradient
+        XSG_REQUIRE(std::isfinite(float(s.lr)) && std::isfinite(float(s.lr * s.weight_decay)),
+                    "adamw_update: learning rate, or its product with the weight decay, beyond 32 bits");
     }
     return XSG_OK;
 }
