@@ -856,3 +856,15 @@ def test_operators_stand_outside_autograd():
     assert not X.adamw_update_([p], [g], [m], [v], X.adamw_step_counter("cuda"), lr=0.1, max_norm=1.0).requires_grad
     for f in (X.gradient_norm, X.clip_gradients_, X.adamw_update_):
         assert "outside autograd" in " ".join(f.__doc__.split())
+
+
+@pytest.mark.parametrize("eps", [1e-45, 1e-46, 1e-60, 1e-300])
+def test_adamw_eps_below_32_bits(eps):
+    # 0 / (0 + eps) is 0 for every eps above 0: an entry without gradient keeps its parameter
+    p, m, v = make([3000], torch.float32, 1), make([3000], torch.float32, 2), make([3000], torch.float32, 3)
+    g = [torch.zeros(3000, device="cuda")]
+    m[0].zero_()
+    v[0].zero_()
+    before = p[0].clone()
+    X.adamw_update_(p, g, m, v, X.adamw_step_counter("cuda"), lr=0.1, eps=eps)
+    assert torch.equal(p[0], before)

@@ -32,6 +32,7 @@
 #include <cmath>
 #include <cstring>
 #include <exception>
+#include <limits>
 #include <type_traits>
 #include <vector>
 
@@ -1280,7 +1281,8 @@ AdamHyper hyper_of(const xsg_adamw_span& s) {
     h.rest2 = float(1.0 - s.beta2);
     h.lr = float(s.lr);
     h.lr_decay = float(s.lr * s.weight_decay);
-    h.eps = float(s.eps);
+    // an eps above 0 stays above 0, so that an entry that never had a gradient gives 0 / eps = 0, not NaN
+    h.eps = s.eps > 0 ? std::max(float(s.eps), std::numeric_limits<float>::denorm_min()) : 0.f;
     h.log_beta1 = float(std::log(s.beta1));
     h.log_beta2 = float(std::log(s.beta2));
     return h;
