@@ -531,7 +531,8 @@ void xsg_exchange_set_max_ctas(int n);
  * returns; the tensors they point to are on the device, dense (any order of
  * dimensions, no gaps), aligned to their element, and may be of any length,
  * zero included.  The sum of all lengths is below 2^40.  Sums are held in 64
- * bits and taken in an order that depends on the lengths alone. */
+ * bits and taken in an order that depends on the lengths and on the tensors'
+ * addresses modulo 128 bytes alone. */
 enum xsg_dtype {
     XSG_F32 = 0,
     XSG_BF16 = 1,

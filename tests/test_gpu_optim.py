@@ -868,3 +868,17 @@ def test_adamw_eps_below_32_bits(eps):
     before = p[0].clone()
     X.adamw_update_(p, g, m, v, X.adamw_step_counter("cuda"), lr=0.1, eps=eps)
     assert torch.equal(p[0], before)
+
+
+@pytest.mark.parametrize("p", [2.0, 1.0])
+@pytest.mark.parametrize("offset", [0, 1, 7, 31])
+def test_same_bits_at_the_same_place_in_a_line(offset, p):
+    # sums depend on lengths and on addresses modulo 128 bytes: what ranks have to agree on to agree in the last bit
+    sizes = [1_000_003, 70_001, 400_000]
+    data = make([sum(sizes)], torch.float32, 3)[0]
+    norms = set()
+    for lines in (0, 1, 5):
+        flat = torch.empty(sum(sizes) + 32 * lines + offset, device="cuda")[32 * lines + offset:]
+        flat.copy_(data)
+        norms.add(float(X.gradient_norm(list(flat.split(sizes)), p)))
+    assert len(norms) == 1

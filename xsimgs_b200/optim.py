@@ -17,7 +17,8 @@ functions take them all in one or two launches, without a host round trip:
 
 Tensors are float32, bfloat16 or float16 on one CUDA device; moments and
 masters are float32.  Work is enqueued on the current stream and nothing is
-read back.  Results do not depend on the run: sums are taken in a fixed order.
+read back.  Results do not depend on the run: sums are taken in an order that
+goes by the tensors' sizes and addresses modulo 128 bytes.
 """
 from __future__ import annotations
 
@@ -77,7 +78,8 @@ def adamw_update_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     were.  With either, the norm before clipping is returned.  `masters`:
     32-bit parameters that half-precision `params` are roundings of; both are
     written.  `row_mask` (bool, one entry for each row of dimension 0; one for
-    all tensors or a list): rows with False keep parameter and moments.
+    all tensors or a list): rows with False keep parameter and moments; the
+    norm is of all gradients, theirs too.
 
     Written tensors must be dense and may not share memory; moments and
     masters have their parameter's sizes and order of dimensions.  A gradient
