@@ -882,3 +882,82 @@ def test_same_bits_at_the_same_place_in_a_line(offset, p):
         flat.copy_(data)
         norms.add(float(X.gradient_norm(list(flat.split(sizes)), p)))
     assert len(norms) == 1
+
+
+# ------------------------------- forms of the masked and mixed-type update --
+KINDS = {  # parameter, gradient, master
+    "f32": (torch.float32, torch.float32, False), "bf16": (torch.bfloat16, torch.bfloat16, False),
+    "f16": (torch.float16, torch.float16, False), "bf16_master": (torch.bfloat16, torch.bfloat16, True),
+    "f16_master": (torch.float16, torch.float16, True), "f32_f16grad": (torch.float32, torch.float16, False),
+    "bf16_f32grad_master": (torch.bfloat16, torch.float32, True), "f16_bf16grad": (torch.float16, torch.bfloat16, False),
+}
+
+
+@pytest.mark.parametrize("name", ["some_empty", "vector_edges", "tile_edges", "leaves", "many"])
+@pytest.mark.parametrize("kind", ["f16_master", "f32_f16grad", "bf16_f32grad_master", "f16_bf16grad"])
+@pytest.mark.parametrize("clip", [False, True])
+def test_adamw_more_types(name, kind, clip):
+    dtype, gdtype, mastered = KINDS[kind]
+    p, g, m, v, masters = state_for(SIZE_SETS[name], dtype, 19, gdtype, mastered)
+    old = [tuple(x.clone() for x in q) for q in zip(masters or p, g, m, v)]
+    norm = norm64(g, 2)
+    got = X.adamw_update_(p, g, m, v, X.adamw_step_counter("cuda", 4), lr=2e-3, weight_decay=0.02,
+                          max_norm=0.2 * norm if clip else None, masters=masters)
+    check_update(p, g, m, v, masters, old, 5, [2e-3] * len(p), (0.9, 0.999), 1e-8, 0.02,
+                 0.2 * norm / (norm + CLIP_EPS) if clip else 1.0)
+    assert got is None or abs(float(got) - norm) <= 10 * U * norm
+
+
+@pytest.mark.parametrize("shape", [(3, 1), (5, 2), (1001, 2), (301, 3), (203, 5), (5, 16383), (5, 16384), (3, 20011),
+                                   (2, 140_001), (40_000, 2), (30_011, 3), (60_001, 1), (7001, 48)])
+@pytest.mark.parametrize("offsets", [(0, 0, 0, 0), (1, 1, 1, 1), (7, 7, 7, 7), (37, 37, 37, 37), (0, 1, 2, 3)])
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("clip", [False, True])
+def test_adamw_rows_at_offsets(shape, offsets, kind, clip):
+    dtype, gdtype, mastered = KINDS[kind]
+    n = math.prod(shape)
+    p, g, m, v, masters = state_for([n + 64], dtype, 43, gdtype, mastered)
+    whole = [p[0], g[0], m[0], v[0]] + ([masters[0]] if mastered else [])
+    kept = [x.clone() for x in whole]
+    places = list(offsets) + ([offsets[0]] if mastered else [])
+    views = [[x[o:o + n].view(shape)] for x, o in zip(whole, places)]
+    p, g, m, v = views[:4]
+    masters = views[4] if mastered else None
+    mask = torch.rand(shape[0], generator=torch.Generator().manual_seed(7)).lt(0.5).cuda()
+    old = [tuple(x[0].clone() for x in (masters or p, g, m, v))]
+    bits = p[0].clone()
+    norm = norm64(g, 2)
+    X.adamw_update_(p, g, m, v, X.adamw_step_counter("cuda", 9), lr=0.01, row_mask=mask, masters=masters,
+                    max_norm=0.5 * norm if clip else None)
+    check_update(p, g, m, v, masters, old, 10, [0.01], (0.9, 0.999), 1e-8, 0.0,
+                 0.5 * norm / (norm + CLIP_EPS) if clip else 1.0, [mask])
+    assert torch.equal(p[0][~mask], bits[~mask])
+    for x, k, o in zip(whole, kept, places):  # the bytes around each view
+        assert torch.equal(x[:o], k[:o]) and torch.equal(x[o + n:], k[o + n:])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16_master"])
+@pytest.mark.parametrize("clip", [False, True])
+def test_adamw_rows_large_at_offsets(kind, clip):
+    # more tiles than blocks, tensors masked and not, at offsets of their own in one buffer for each array
+    dtype, gdtype, mastered = KINDS[kind]
+    shapes = [(1_000_003, 3), (1_000_003,), (400_001, 2), (129, 20_011), (300_007,)]
+    sizes = [math.prod(s) for s in shapes]
+    flat = state_for([sum(sizes) + 5], dtype, 47, gdtype, mastered)
+
+    def split(x):
+        return [y.view(s) for y, s in zip(x[0][5:].split(sizes), shapes)]
+
+    p, g, m, v = (split(x) for x in flat[:4])
+    masters = split(flat[4]) if mastered else None
+    masks = [torch.rand(s[0], generator=torch.Generator().manual_seed(i)).lt(0.4).cuda() if i != 4 else None
+             for i, s in enumerate(shapes)]
+    old = [tuple(x.clone() for x in q) for q in zip(masters or p, g, m, v)]
+    bits = [x.clone() for x in p]
+    norm = norm64(g, 2)
+    X.adamw_update_(p, g, m, v, X.adamw_step_counter("cuda", 9), lr=0.01, row_mask=masks, masters=masters,
+                    max_norm=0.5 * norm if clip else None)
+    check_update(p, g, m, v, masters, old, 10, [0.01] * 5, (0.9, 0.999), 1e-8, 0.0,
+                 0.5 * norm / (norm + CLIP_EPS) if clip else 1.0, masks)
+    for x, b, mask in zip(p, bits, masks):
+        assert mask is None or torch.equal(x[~mask], b[~mask])
