@@ -667,7 +667,8 @@ __device__ __forceinline__ void adam_element(const AdamScale& h, float g, float&
     // A moment whose gradients have long been zero stays among the subnormal
     // numbers, on which a division takes a slow path (59 M of them: 326 us
     // against 272); a product does not.  The reciprocal is exact to half an
-    // ulp and finite from 2^-126 on.
+    // ulp and finite from 2^-126 on; the limit leaves that a wide margin, and
+    // only an eps below 1e-30 lets a denominator under it.
     const float q = den >= 0x1p-100f ? m * __frcp_rn(den) : m / den;
     w -= h.step_size * q;
 }
